@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libnative_hip.so")
-SOURCES = ["kernels.hip", "executor.cpp", "residency.cpp", "gguf.cpp", "llama_host.cpp"]
+SOURCES = ["kernels.hip", "attn.hip", "executor.cpp", "residency.cpp", "gguf.cpp", "llama_host.cpp"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # packed-FP32 VALU forms are kept out of every kernel
@@ -70,6 +70,26 @@ def build_selftest(verbose=False):
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     return SELFTEST_BIN
+
+
+class KvCache(C.Structure):
+    """A paged K/V cache in the caller's device memory (lnh_kv_cache, include/native_hip_attention.h): k and v as
+    [n_blocks][n_layer][n_head_kv][kv_block][head_dim] of F32 or F16, w (0: none) the same without the last axis, f32."""
+    _fields_ = [(n, C.c_uint32) for n in ("ggml_type", "n_layer", "n_head_kv", "head_dim", "kv_block", "n_blocks")] + \
+               [(n, C.c_void_p) for n in ("device_k", "device_v", "device_w")]
+
+    def __init__(self, ggml_type, n_layer, n_head_kv, head_dim, kv_block, n_blocks, k_ptr, v_ptr, w_ptr=0):
+        super().__init__(ggml_type, n_layer, n_head_kv, head_dim, kv_block, n_blocks, k_ptr, v_ptr, w_ptr)
+
+
+class KvSeqs(C.Structure):
+    """The sequences of a call (lnh_kv_seqs): tables [n_seqs][table_stride], lens [n_seqs] and starts [n_seqs + 1]
+    (0: one new token each) are u32 arrays in device memory; lens counts the new tokens."""
+    _fields_ = [(n, C.c_size_t) for n in ("n_seqs", "n_tokens", "max_new", "max_len")] + \
+               [("device_tables", C.c_void_p), ("table_stride", C.c_size_t), ("device_lens", C.c_void_p), ("device_starts", C.c_void_p)]
+
+    def __init__(self, n_seqs, tables_ptr, table_stride, lens_ptr, max_len, starts_ptr=0, n_tokens=None, max_new=1):
+        super().__init__(n_seqs, n_seqs if n_tokens is None else n_tokens, max_new, max_len, tables_ptr, table_stride, lens_ptr, starts_ptr)
 
 
 _lib = None
@@ -161,10 +181,17 @@ def load_library():
         "lnm_gguf_tensor": (C.c_int, [vp, sz, sz, C.c_char_p, sz, C.POINTER(u32), C.POINTER(C.c_uint64),
                                       C.POINTER(u32), psz, psz]),
     }
-    for name, (res, args) in sig.items():
+    # include/native_hip_attention.h
+    pc, ps = C.POINTER(KvCache), C.POINTER(KvSeqs)
+    paged = {
+        "lnh_kv_store_device": (C.c_int, [vp, pc, ps, sz, vp, sz, vp, sz, vp]),
+        "lnh_attn_device": (C.c_int, [vp, pc, ps, sz, sz, vp, sz, vp, sz, C.c_float, sz, sz, C.c_int, C.c_float, vp]),
+        "lnh_kv_evict_device": (C.c_int, [vp, pc, ps, sz, sz, sz, sz, sz, vp, sz, vp, vp]),
+    }
+    for name, (res, args) in list(sig.items()) + list(paged.items()):
         fn = getattr(lib, name)  # AttributeError if the ABI lost a symbol
         fn.restype, fn.argtypes = res, args
-    lib._signatures = sig
+    lib._signatures, lib._paged_signatures = sig, paged
     _lib = lib
     return lib
 
@@ -429,6 +456,25 @@ class HipGemv:
         """h = SiLU(gate x') * (up x') in one launch; x' = x or RMSNorm(x) * x2."""
         self._check(self._lib.lnh_gemv_swiglu_device(self._h, gate._h, up._h, C.c_void_p(x_ptr), C.c_void_p(h_ptr),
                                                      prologue, C.c_void_p(x2_ptr), eps, C.c_void_p(stream)))
+
+    def kv_store_device(self, cache, seqs, layer, k_ptr, v_ptr, k_stride=None, v_stride=None, stream=0):
+        """K and V of the new tokens into the cache; strides in floats, None: rows back to back."""
+        row = cache.n_head_kv * cache.head_dim
+        self._check(self._lib.lnh_kv_store_device(self._h, C.byref(cache), C.byref(seqs), layer, k_ptr, row if k_stride is None else k_stride,
+                                                  v_ptr, row if v_stride is None else v_stride, stream))
+
+    def attn_device(self, cache, seqs, layer, n_head, q_ptr, out_ptr, scale, q_stride=None, out_stride=None, window=0, sinks=0,
+                    weights=False, decay=1.0, stream=0):
+        """out = softmax(scale q K^T) V of the new tokens; window > 0: the last `window` positions and the first `sinks`;
+        weights: the cache's w = decay * w + the probabilities of this call."""
+        row = n_head * cache.head_dim
+        self._check(self._lib.lnh_attn_device(self._h, C.byref(cache), C.byref(seqs), layer, n_head, q_ptr, row if q_stride is None else q_stride,
+                                              out_ptr, row if out_stride is None else out_stride, scale, window, sinks, int(weights), decay, stream))
+
+    def kv_evict_device(self, cache, seqs, first_layer, n_layers, keep, first, recent, dst_tables_ptr, dst_stride, new_lens_ptr, stream=0):
+        """Every sequence to at most `keep` positions: the first, the recent, the heaviest between; dst_tables_ptr 0: in place."""
+        self._check(self._lib.lnh_kv_evict_device(self._h, C.byref(cache), C.byref(seqs), first_layer, n_layers, keep, first, recent,
+                                                  dst_tables_ptr, dst_stride, new_lens_ptr, stream))
 
     def calibration_copy(self, dst_ptr, src_ptr, nbytes, stream=0):
         self._check(self._lib.lnh_calibration_copy(self._h, C.c_void_p(dst_ptr), C.c_void_p(src_ptr), nbytes,

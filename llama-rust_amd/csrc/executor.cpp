@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/native_hip.h"
+#include "attn.h"
 #include "early_gemm.h"
 #include "head_step.h"
 #include "host_range.h"
@@ -172,7 +173,8 @@ bool ensure_pinned(lnh_exec *e, size_t in_floats, size_t out_floats) {
 // while another call, a longer prompt say, makes the workspace grow), and work already queued may still use
 // it.  Growth is by at least half, so everything retired together is smaller than twice the live buffer.
 // `least`: what the call can do with (more slowly) where `bytes` cannot be had.
-int ensure_workspace(lnh_exec *e, hipStream_t s, size_t bytes, size_t least) {
+constexpr const char *GROW_BEFORE_PRODUCTS = "run the largest product once before capturing, or use lnh_gemm_device_noalloc";
+int ensure_workspace(lnh_exec *e, hipStream_t s, size_t bytes, size_t least, const char *instead = GROW_BEFORE_PRODUCTS) {
     if (bytes <= e->ws_cap) return LNH_OK;
     // Growing allocates, which a stream under capture cannot record: refuse before anything is launched
     // instead of leaving the caller with a broken capture.
@@ -180,9 +182,7 @@ int ensure_workspace(lnh_exec *e, hipStream_t s, size_t bytes, size_t least) {
     if (s && hipStreamIsCapturing(s, &capturing) == hipSuccess && capturing != hipStreamCaptureStatusNone) {
         if (least <= e->ws_cap) return LNH_OK;
         return fail(e, LNH_ERR_INVALID,
-                    "the multi-token workspace must grow to " + std::to_string(bytes) +
-                        " bytes while the stream is being captured: run the largest product once before capturing, "
-                        "or use lnh_gemm_device_noalloc");
+                    "the multi-token workspace must grow to " + std::to_string(bytes) + " bytes while the stream is being captured: " + instead);
     }
     (void)hipGetLastError();
     const size_t grown = bytes > e->ws_cap + e->ws_cap / 2 ? bytes : e->ws_cap + e->ws_cap / 2;
@@ -1184,3 +1184,5 @@ size_t lnh_resident_bytes(uint32_t type, size_t rows, size_t cols, size_t tokens
 }
 
 }  // extern "C"
+
+#include "attn_exec.inc"

@@ -9,6 +9,7 @@ namespace nh {
 // CU count and the largest dynamic LDS a workgroup may ask for on this device.  Held once per process: the
 // first call sets them, a later call returns false when its values differ (the caller refuses the executor).
 bool set_device_limits(int cu_count, size_t lds_per_block);
+int device_cu_count();
 
 // What the device's converts give for nibble bytes: the value of byte 0x01 under the fp8 (E4M3) unpack when bytes
 // 0..15 decode linearly (n * unit, a power of two), else 0 (nibble kernels then take the byte-convert path);

@@ -58,6 +58,7 @@ bool set_device_limits(int cu_count, size_t lds_per_block) {
     g_limits_set = true;
     return true;
 }
+int device_cu_count() { return g_cu_count; }
 
 template <uint32_t T, int LB, int R, int K, bool SPLIT>
 static hipError_t launch_rows(hipStream_t stream, const MatView *mats, float *const *ys, uint32_t n_jobs, const float *x, bool accumulate) {

@@ -1,0 +1,491 @@
+"""Operators over the paged K/V cache on the GPU against their definition in 64 bits (tests/paged.py): types, head layouts,
+lengths from none to thousands, windows, tables that name no block, infinities where nobody looks, graphs, streams."""
+import importlib
+
+import numpy as np
+import pytest
+
+from paged import NOWHERE, Paged, same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def gpu(pkg):
+    g = pkg.HipGemv(0)
+    yield g
+    g.close()
+
+
+@pytest.fixture(scope="module")
+def hip():
+    return importlib.import_module("llama-rust_amd.hiprt")
+
+
+def attend(gpu, c, layer, q, scale, out=None, q_stride=None, out_stride=None, stream=0, **kw):
+    """The call, synchronised; out keeps what it held in rows the call leaves alone."""
+    hip = c.hip
+    dq = hip.DeviceBuffer.from_numpy(q.astype(np.float32))
+    start = np.full(q.shape, 7.25, np.float32) if out is None else out
+    do = hip.DeviceBuffer.from_numpy(start)
+    gpu.attn_device(c.cache, c.seqs, layer, kw.pop("heads", q.shape[-2]), dq.ptr, do.ptr, scale, q_stride=q_stride, out_stride=out_stride, stream=stream, **kw)
+    hip.device_synchronize()
+    return do.to_numpy(np.float32).reshape(start.shape)
+
+
+def check(got, want, tol, what=""):
+    assert np.all(np.isfinite(got)), what
+    off = np.abs(got.astype(np.float64) - want)
+    worst = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert np.all(off <= tol), (what, worst, got[worst], want[worst], tol[worst])
+
+
+LAYOUTS = [(1, 1, 64), (4, 4, 128), (8, 2, 128), (14, 2, 64), (32, 4, 80), (6, 2, 40), (3, 1, 8), (16, 1, 256), (12, 4, 192), (71, 1, 64), (34, 2, 136)]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("heads,hkv,d", LAYOUTS)
+def test_one_token_a_sequence(gpu, f16, heads, hkv, d):
+    """Lengths around the tiles' and blocks' ends, a sequence that holds nothing, blocks of sixteen."""
+    rng = np.random.default_rng(d + heads)
+    c = Paged(rng, f16, 2, hkv, d, 16, [1, 0, 15, 16, 17, 33, 64, 130, 300]).up()
+    q = rng.normal(0, 1, (9, heads, d)).astype(np.float32)
+    want, tol, _ = c.attend(1, q, d ** -0.5)
+    got = attend(gpu, c, 1, q, np.float32(d ** -0.5))
+    check(got, want, tol + 1e-7 * np.abs(want))
+    assert np.all(got[1] == 0)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("block", [1, 3, 16, 20, 48, 256])
+def test_blocks_of_any_size(gpu, f16, block):
+    rng = np.random.default_rng(block)
+    c = Paged(rng, f16, 3, 2, 64, block, [5, 257, 100]).up()
+    q = rng.normal(0, 1, (3, 4, 64)).astype(np.float32)
+    want, tol, _ = c.attend(2, q, 0.125)
+    check(attend(gpu, c, 2, q, 0.125), want, tol)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_long_sequences_are_shared_and_joined(gpu, f16):
+    """Lengths that are cut into many shares, beside one that leaves most shares empty; large scores in one place, so that a row's
+    maximum rises late."""
+    rng = np.random.default_rng(3)
+    c = Paged(rng, f16, 1, 2, 64, 32, [5000, 40, 2999])
+    c.k[c.at(0, 4000)] *= 20
+    c.k[c.at(2, 3)] *= 20
+    c.up()
+    q = rng.normal(0, 1, (3, 8, 64)).astype(np.float32)
+    want, tol, _ = c.attend(0, q, 0.125)
+    check(attend(gpu, c, 0, q, 0.125), want, tol)
+
+
+RAGGED = [([0, 1, 4, 4, 21, 22], [1, 3, 9, 17, 60]), ([0, 40, 41, 105, 105, 170], [40, 90, 64, 5, 200])]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("starts,lens", RAGGED)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (7, 0), (7, 3), (40, 4), (1000, 4), (30, 50)])
+def test_several_tokens_a_sequence(gpu, f16, starts, lens, window, sinks):
+    """Prompts and remainders of any length, one of them without new tokens; causal, in a window, with first tokens."""
+    rng = np.random.default_rng(window + sinks)
+    c = Paged(rng, f16, 2, 2, 64, 16, lens).up(starts, max_new=int(np.diff(starts).max()))
+    q = rng.normal(0, 1, (starts[-1], 6, 64)).astype(np.float32)
+    want, tol, _ = c.attend(0, q, 0.125, starts, window, sinks)
+    check(attend(gpu, c, 0, q, 0.125, window=window, sinks=sinks), want, tol)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("heads,hkv,d,block", [(4, 4, 128, 16), (8, 1, 256, 20), (10, 2, 96, 16), (40, 2, 40, 7), (9, 1, 192, 64)])
+def test_prompts_in_other_layouts(gpu, f16, heads, hkv, d, block):
+    rng = np.random.default_rng(d)
+    starts = [0, 33, 34, 120]
+    c = Paged(rng, f16, 1, hkv, d, block, [33, 50, 150]).up(starts, max_new=86)
+    q = rng.normal(0, 1, (120, heads, d)).astype(np.float32)
+    for window, sinks in ((0, 0), (20, 4)):
+        want, tol, _ = c.attend(0, q, d ** -0.5, starts, window, sinks)
+        check(attend(gpu, c, 0, q, np.float32(d ** -0.5), window=window, sinks=sinks), want, tol + 1e-7 * np.abs(want))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_rows_apart_and_rows_of_nobody(gpu, f16):
+    """Strides wider than a row; rows before the first sequence and behind the last stay as they were."""
+    rng = np.random.default_rng(11)
+    starts = [2, 3, 8]
+    c = Paged(rng, f16, 1, 2, 64, 16, [30, 44]).up(starts, max_new=5, n_tokens=11)
+    q = np.full((11, 300), np.nan, np.float32)
+    q[:, :256] = rng.normal(0, 1, (11, 256))
+    out = rng.normal(0, 1, (11, 272)).astype(np.float32)
+    got = attend(gpu, c, 0, q, 0.125, out=out.copy(), q_stride=300, out_stride=272, heads=4)
+    want, tol, _ = c.attend(0, q[:, :256].reshape(11, 4, 64), 0.125, starts)
+    check(got[2:8, :256].reshape(6, 4, 64), want[2:8], tol[2:8])
+    assert np.array_equal(got[:2], out[:2]) and np.array_equal(got[8:], out[8:]) and np.array_equal(got[:, 256:], out[:, 256:])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_no_row_sees_reaches_none(gpu, f16, bad):
+    """Infinities and NaN behind the length, before the window, in a later token of the same call."""
+    rng = np.random.default_rng(5)
+    starts = [0, 20, 21]
+    c = Paged(rng, f16, 1, 2, 64, 16, [50, 90], garbage=bad)
+    for x in (c.k, c.v):
+        x[c.at(0, 41)] = bad  # token 11 of the first sequence
+        x[c.at(1, 20)] = bad  # outside the second one's window
+    c.up(starts, max_new=20)
+    q = rng.normal(0, 1, (21, 4, 64)).astype(np.float32)
+    got = attend(gpu, c, 0, q, 0.125, window=30, sinks=4)
+    want, tol, _ = c.attend(0, q, 0.125, starts, 30, 4)
+    check(got[:11], want[:11], tol[:11])
+    check(got[20:], want[20:], tol[20:])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_infinities_that_are_seen(gpu, f16):
+    """As the definition has them: a score of -infinity counts nothing, all of them leave zeros, an infinite value passes, +infinity and NaN
+    in a score are NaN."""
+    rng = np.random.default_rng(6)
+    c = Paged(rng, f16, 1, 1, 64, 16, [40] * 5)
+    q = np.abs(rng.normal(0, 1, (5, 2, 64))).astype(np.float32) + 0.1
+    c.k[c.at(0, 7)] = -np.inf
+    for t in range(40):
+        c.k[c.at(1, t)] = -np.inf
+    c.v[c.at(2, 30)] = np.inf
+    c.k[c.at(3, 9)] = np.inf
+    c.k[c.at(4, 9)] = np.nan
+    c.up()
+    got = attend(gpu, c, 0, q, 0.125)
+    want, tol, _ = c.attend(0, q, 0.125)
+    check(got[0], want[0], tol[0])
+    assert np.all(got[1] == 0)
+    assert np.all(got[2] == np.inf)
+    assert np.all(np.isnan(got[3])) and np.all(np.isnan(got[4]))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_scores_of_any_size(gpu, f16):
+    """Queries far above and below one: the softmax picks one position, or weighs all alike."""
+    rng = np.random.default_rng(8)
+    c = Paged(rng, f16, 1, 1, 64, 16, [200] * 6).up()
+    q = rng.normal(0, 1, (6, 4, 64)).astype(np.float32) * np.array([1e-38, 1e-30, 1e-3, 30, 1e5, 1e20], np.float32)[:, None, None]
+    want, tol, _ = c.attend(0, q, 0.125)
+    got = attend(gpu, c, 0, q, 0.125)
+    check(got[:4], want[:4], tol[:4])
+    assert np.all(np.isfinite(got))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_blocks_that_are_not_there(gpu, f16):
+    """Entries of a table that name no block are as if their positions were not; a length beyond max_len and row starts out of order stay in
+    bounds."""
+    rng = np.random.default_rng(9)
+    c = Paged(rng, f16, 2, 2, 64, 16, [70, 16, 120])
+    c.tables[0, 1] = c.n_blocks
+    c.tables[1, 0] = NOWHERE
+    c.tables[2, 3] = 0x80000000
+    c.up()
+    q = rng.normal(0, 1, (3, 4, 64)).astype(np.float32)
+    want, tol, _ = c.attend(1, q, 0.125)
+    got = attend(gpu, c, 1, q, 0.125)
+    check(got, want, tol)
+    assert np.all(got[1] == 0)
+    c.lens = np.array([70, 16, 100], np.uint32)
+    c.dl.upload(np.array([70, 16, 1 << 30], np.uint32))
+    c.seqs.max_len = 100
+    want, tol, _ = c.attend(1, q, 0.125)
+    check(attend(gpu, c, 1, q, 0.125), want, tol)
+    c.up([0, 3, 1, 90], max_new=2, n_tokens=3, max_len=100)
+    got = attend(gpu, c, 1, q, 0.125)
+    assert np.all(np.isfinite(got))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("decay", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("starts,lens,window,sinks", [(None, [1, 0, 31, 64, 700], 0, 0), ([0, 40, 41, 105, 105, 170], [40, 90, 64, 5, 200], 0, 0),
+                                                       ([0, 3, 60], [90, 57], 25, 4)])
+def test_weights_are_summed(gpu, f16, decay, starts, lens, window, sinks):
+    rng = np.random.default_rng(len(lens))
+    news = np.diff(starts) if starts else [1]
+    c = Paged(rng, f16, 2, 2, 64, 16, lens, weights=True).up(starts, max_new=int(max(news)))
+    q = rng.normal(0, 1, (starts[-1] if starts else len(lens), 6, 64)).astype(np.float32)
+    want, tol, sums = c.attend(1, q, 0.125, starts, window, sinks)
+    got = attend(gpu, c, 1, q, 0.125, window=window, sinks=sinks, weights=True, decay=decay)
+    check(got, want, tol)
+    w, w_tol = c.weigh(1, sums, decay)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert same_bits(after[~held], c.w[~held])
+    off = np.abs(after[held] - w[held])
+    assert np.all(off <= w_tol[held]), np.max(off - w_tol[held])
+
+
+def test_weights_do_not_change_the_output(gpu):
+    rng = np.random.default_rng(2)
+    for starts in (None, [0, 30, 70]):
+        c = Paged(rng, True, 1, 2, 64, 16, [300, 500], weights=True).up(starts, max_new=40 if starts else 1)
+        q = rng.normal(0, 1, (70 if starts else 2, 8, 64)).astype(np.float32)
+        assert np.array_equal(attend(gpu, c, 0, q, 0.125), attend(gpu, c, 0, q, 0.125, weights=True))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_store(gpu, hip, f16):
+    """Rows of several sequences with strides of their own, into blocks that exist; nothing else is touched."""
+    rng = np.random.default_rng(4)
+    starts = [1, 4, 4, 30, 31, 33]
+    lens = [5, 9, 40, 1, 1]  # the last has more new tokens than positions
+    c = Paged(rng, f16, 2, 3, 40, 7, lens, garbage=-1.0)
+    c.tables[2, 3] = c.n_blocks + 5
+    c.up(starts, max_new=26, n_tokens=35, max_len=40)
+    k, v = rng.normal(0, 1, (35, 124)).astype(np.float32), rng.normal(0, 1, (35, 160)).astype(np.float32)
+    k[5, :4] = [1e-9, 65519.0, 65520.0, -1e9]
+    k[6, 0], k[6, 1] = np.inf, np.nan
+    dk, dv = hip.DeviceBuffer.from_numpy(k), hip.DeviceBuffer.from_numpy(v)
+    gpu.kv_store_device(c.cache, c.seqs, 1, dk.ptr, dv.ptr, k_stride=124, v_stride=160)
+    hip.device_synchronize()
+    want_k, want_v = c.k.copy(), c.v.copy()
+    with np.errstate(over="ignore"):
+        for b, (n0, n1) in enumerate(zip(starts, starts[1:])):
+            for i in range(n1 - n0):
+                t = lens[b] - (n1 - n0) + i
+                if t < 0 or not c.there(b, t):
+                    continue
+                want_k[c.tables[b, t // 7], 1, :, t % 7] = k[n0 + i, :120].reshape(3, 40).astype(want_k.dtype)
+                want_v[c.tables[b, t // 7], 1, :, t % 7] = v[n0 + i, :120].reshape(3, 40).astype(want_v.dtype)
+    got_k, got_v, _ = c.down()
+    assert same_bits(got_k, want_k) and same_bits(got_v, want_v)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("keep,first,recent", [(40, 4, 8), (40, 0, 0), (40, 20, 20), (1, 0, 0), (1, 0, 1), (0, 0, 0), (129, 4, 100), (5000, 4, 4)])
+def test_eviction(gpu, hip, f16, in_place, keep, first, recent):
+    """Lengths below, at and above the budget; ties, zeros of both signs, infinities and NaN among the weights; a block missing."""
+    rng = np.random.default_rng(keep + first)
+    lens = [1, 0, 39, 40, 41, 128, 300, 3000]
+    c = Paged(rng, f16, 3, 2, 40, 16, lens, weights=True, garbage=-3.0, extra_blocks=sum(-(-min(n, keep) // 16) for n in lens))
+    for t in range(0, 300, 3):
+        c.w[c.at(6, t)] = np.float32(0.5)
+    for t, x in ((10, np.nan), (11, np.inf), (12, -0.0), (13, 0.0), (14, -1.0), (15, -np.inf), (16, np.float32(1e-42))):
+        c.w[c.at(5, t)] = x
+    c.w[c.at(7, 0)] = 0
+    for t in range(500, 2500):
+        c.w[c.at(7, t)] = np.float32(rng.integers(0, 3))
+    c.tables[6, 5] = NOWHERE
+    dst, at = None, 0
+    if not in_place:
+        stride = max(1, -(-min(keep, 3000) // 16))
+        dst = np.full((len(lens), stride), NOWHERE, np.uint32)
+        for b, n in enumerate(lens):
+            pages = -(-min(n, keep) // 16)
+            dst[b, :pages] = c.free[at:at + pages]
+            at += pages
+    c.up()
+    dd = hip.DeviceBuffer.from_numpy(dst) if dst is not None else None
+    new = c.dl if in_place else hip.DeviceBuffer(4 * len(lens))
+    gpu.kv_evict_device(c.cache, c.seqs, 1, 2, keep, first, recent, dd.ptr if dd else 0, dst.shape[1] if dd else 0, new.ptr)
+    hip.device_synchronize()
+    want_len, k, v, w = c.evict([1, 2], keep, first, recent, dst)
+    got_k, got_v, got_w = c.down()
+    assert np.array_equal(new.to_numpy(np.uint32), want_len)
+    if in_place:  # what lies behind the new lengths may be anything that was there
+        for b, n in enumerate(want_len.astype(int)):
+            for t in range(n):
+                if c.there(b, t):
+                    at = c.at(b, t)
+                    assert same_bits(got_k[at], k[at]) and same_bits(got_v[at], v[at]) and same_bits(got_w[at], w[at]), (b, t)
+        assert same_bits(got_k[:, 0], c.k[:, 0]) and same_bits(got_w[c.free], c.w[c.free])
+    assert same_bits(got_k, k) and same_bits(got_v, v) and same_bits(got_w, w)
+
+
+def test_a_cache_of_more_than_four_gigabytes(gpu, hip, pkg):
+    """Rows whose offset does not fit 32 bits, in elements or bytes."""
+    rng = np.random.default_rng(1)
+    d, block, n_blocks = 256, 64, 300000  # 4.9e9 elements
+    size = n_blocks * block * d * 2
+    dk, dv, dw = hip.DeviceBuffer(size), hip.DeviceBuffer(size), hip.DeviceBuffer(n_blocks * block * 4)
+    table = np.array([[299999, 3, 280001, 270000]], np.uint32)
+    dt, dl = hip.DeviceBuffer.from_numpy(table), hip.DeviceBuffer.from_numpy(np.array([180], np.uint32))
+    cache = pkg.KvCache(pkg.F16, 1, 1, d, block, n_blocks, dk.ptr, dv.ptr, dw.ptr)
+    starts = hip.DeviceBuffer.from_numpy(np.array([0, 180], np.uint32))
+    seqs = pkg.KvSeqs(1, dt.ptr, 4, dl.ptr, 180, starts.ptr, 180, 180)
+    k, v, q = (rng.normal(0, 1, (180, d)).astype(np.float32) for _ in range(3))
+    bk, bv, bq = (hip.DeviceBuffer.from_numpy(x) for x in (k, v, q))
+    gpu.kv_store_device(cache, seqs, 0, bk.ptr, bv.ptr)
+    out = hip.DeviceBuffer(180 * d * 4)
+    gpu.attn_device(cache, seqs, 0, 1, bq.ptr, out.ptr, 0.0625, weights=True, decay=0.0)
+    hip.device_synchronize()
+    k16, v16 = k.astype(np.float16).astype(np.float64), v.astype(np.float16).astype(np.float64)
+    s = np.where(np.tri(180, dtype=bool), (q.astype(np.float64) @ k16.T) * 0.0625, -np.inf)
+    p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    size = (np.abs(q) @ np.abs(k16).T).max() * 0.0625
+    rel = (2 * (d + 24) * size + 260) * 2.0 ** -23
+    check(out.to_numpy(np.float32).reshape(180, d), p @ v16, rel * (p @ np.abs(v16)))
+    new = hip.DeviceBuffer(4)
+    gpu.kv_evict_device(cache, seqs, 0, 1, 60, 4, 16, 0, 0, new.ptr)
+    one = pkg.KvSeqs(1, dt.ptr, 4, new.ptr, 60)
+    gpu.attn_device(cache, one, 0, 1, bq.ptr, out.ptr, 0.0625)
+    hip.device_synchronize()
+    assert new.to_numpy(np.uint32)[0] == 60
+    w = p.sum(0)
+    order = np.argsort(-w[4:164], kind="stable")
+    assert w[4 + order[39]] - w[4 + order[40]] > 1e-4 * w[4 + order[39]]  # the weights' own error decides nothing here
+    stays = np.concatenate([np.arange(4), np.sort(4 + order[:40]), np.arange(164, 180)])
+    s = (q[:1].astype(np.float64) @ k16[stays].T) * 0.0625
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    check(out.to_numpy(np.float32)[:d][None], p @ v16[stays], rel * (p @ np.abs(v16[stays])))
+
+
+def test_a_decode_loop_with_an_eviction(gpu, hip):
+    """Prompt, tokens one at a time, a cut, tokens again: store, attention with weights and eviction as a program chains them, on a stream of
+    its own, against the definition step by step."""
+    rng = np.random.default_rng(12)
+    lens0 = [20, 1, 33]
+    c = Paged(rng, True, 1, 2, 64, 16, lens0, room=40, weights=True, garbage=0.0)
+    stream = hip.Stream()
+
+    def step(news, lens):
+        starts = np.concatenate([[0], np.cumsum(news)])
+        n, q = int(starts[-1]), rng.normal(0, 1, (int(starts[-1]), 4, 64)).astype(np.float32)
+        k, v = (rng.normal(0, 1, (n, 2, 64)).astype(np.float32) for _ in range(2))
+        c.lens = np.array(lens, np.uint32)
+        c.up(starts, max_new=int(max(news)), max_len=int(max(lens)))
+        bk, bv = hip.DeviceBuffer.from_numpy(k), hip.DeviceBuffer.from_numpy(v)
+        hip.device_synchronize()
+        gpu.kv_store_device(c.cache, c.seqs, 0, bk.ptr, bv.ptr, stream=stream.ptr)
+        for b in range(len(lens)):
+            for i in range(news[b]):
+                at = c.at(b, lens[b] - news[b] + i)
+                row = starts[b] + i
+                c.k[at[0], 0, :, at[3]], c.v[at[0], 0, :, at[3]] = k[row].astype(np.float16), v[row].astype(np.float16)
+        got = attend(gpu, c, 0, q, 0.125, stream=stream.ptr, weights=True, decay=1.0)
+        want, tol, sums = c.attend(0, q, 0.125, starts)
+        check(got, want, tol)
+        w, w_tol = c.weigh(0, sums, 1.0)
+        got_k, got_v, got_w = c.down()
+        assert same_bits(got_k, c.k) and same_bits(got_v, c.v)
+        assert np.all(np.abs(got_w - w) <= w_tol)
+        c.w = got_w  # what later steps add to, and the cut goes by
+
+    step(lens0, lens0)
+    lens = list(lens0)
+    for _ in range(6):
+        lens = [n + 1 for n in lens]
+        step([1, 1, 1], lens)
+    c.up(max_len=max(lens))
+    hip.device_synchronize()
+    gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 16, 2, 5, 0, 0, c.dl.ptr, stream=stream.ptr)
+    stream.synchronize()
+    new, c.k, c.v, c.w = c.evict([0], 16, 2, 5)
+    assert np.array_equal(c.dl.to_numpy(np.uint32), new)
+    assert all(same_bits(x, y) for x, y in zip(c.down(), (c.k, c.v, c.w)))
+    lens = [int(n) for n in new]
+    for _ in range(3):
+        lens = [n + 1 for n in lens]
+        step([1, 1, 1], lens)
+    stream.destroy()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 24])
+def test_a_captured_step_follows_its_arrays(gpu, hip, f16, new):
+    """Store, attention with weights and eviction in one graph, replayed with other lengths, tables and values; every replay equals the
+    eager calls bit for bit."""
+    rng = np.random.default_rng(21)
+    starts = [0, new, 2 * new] if new > 1 else None
+    c = Paged(rng, f16, 1, 2, 64, 16, [640, 500], room=16, weights=True, garbage=0.0)
+    c.up(starts, max_new=new, max_len=656)
+    bk, bv, bq, bo, bn = (hip.DeviceBuffer(2 * new * n * 4) for n in (128, 128, 256, 256, 1))
+    stream = hip.Stream()
+
+    def enqueue(s):
+        gpu.kv_store_device(c.cache, c.seqs, 0, bk.ptr, bv.ptr, stream=s.ptr)
+        gpu.attn_device(c.cache, c.seqs, 0, 4, bq.ptr, bo.ptr, 0.125, weights=True, decay=0.5, stream=s.ptr)
+        gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 300, 4, 32, 0, 0, bn.ptr, stream=s.ptr)
+
+    def fill():
+        c.dk.upload(c.k), c.dv.upload(c.v), c.dw.upload(c.w)
+
+    enqueue(stream)  # sizes the workspace
+    stream.synchronize()
+    graph = hip.Graph(stream, enqueue)
+    for lens in ([640, 500], [33, 656], [new, 301], [650, 40]):
+        order = rng.permutation(2)
+        tables = c.tables[order]
+        rows = [rng.normal(0, 1, 2 * new * n).astype(np.float32) for n in (128, 128, 256)]
+        got = []
+        for run in (enqueue, lambda s: graph.launch(), enqueue, lambda s: graph.launch()):
+            fill()
+            c.dt.upload(tables), c.dl.upload(np.array(lens, np.uint32))
+            for b, x in zip((bk, bv, bq), rows):
+                b.upload(x)
+            hip.device_synchronize()
+            run(stream)
+            stream.synchronize()
+            got.append([bo.to_numpy(np.float32), bn.to_numpy(np.uint32, 2)] + list(c.down()))
+        for other in got[1:]:
+            assert all(np.array_equal(x.view(np.uint8), y.view(np.uint8)) for x, y in zip(got[0], other)), lens
+        assert got[0][1].tolist() == [min(n, 300) for n in lens]
+    graph.destroy()
+    stream.destroy()
+
+
+def test_growing_inside_a_capture_is_refused(pkg, hip):
+    g = pkg.HipGemv(0)
+    rng = np.random.default_rng(0)
+    c = Paged(rng, False, 1, 1, 64, 16, [2000], weights=True, garbage=0.0).up()
+    q, o = hip.DeviceBuffer(256), hip.DeviceBuffer(256)
+    stream = hip.Stream()
+    hip.device_synchronize()
+    with pytest.raises(pkg.NativeHipError, match="while the stream is being captured: run the largest call once before capturing"):
+        hip.Graph(stream, lambda s: g.attn_device(c.cache, c.seqs, 0, 1, q.ptr, o.ptr, 0.125, weights=True, stream=s.ptr))
+    g.attn_device(c.cache, c.seqs, 0, 1, q.ptr, o.ptr, 0.125, weights=True, stream=stream.ptr)  # the executor is as usable as before
+    stream.synchronize()
+    stream.destroy()
+    g.close()
+
+
+def test_refusals_name_their_reason_and_touch_nothing(gpu, hip, pkg):
+    rng = np.random.default_rng(0)
+    c = Paged(rng, True, 2, 2, 64, 16, [30], weights=True, garbage=0.0).up()
+    b = hip.DeviceBuffer.from_numpy(np.full(1024, 5, np.float32))
+    o = hip.DeviceBuffer.from_numpy(np.full(1024, 5, np.float32))
+
+    def attn(layer=0, heads=4, q=b.ptr, out=o.ptr, **kw):
+        gpu.attn_device(c.cache, c.seqs, layer, heads, q, out, 0.125, **kw)
+
+    for match, call in (("no such layer", lambda: attn(layer=2)), ("multiple of the key-value heads", lambda: attn(heads=3)),
+                        ("buffer pointer is null", lambda: attn(q=0)), ("16-byte aligned", lambda: attn(out=o.ptr + 4)),
+                        ("less than the row", lambda: attn(q_stride=252)), ("multiples of four", lambda: attn(out_stride=259)),
+                        ("must not be the input", lambda: attn(out=b.ptr)), ("sinks without one", lambda: attn(sinks=4)),
+                        ("scale and decay", lambda: attn(weights=True, decay=float("nan"))),
+                        ("exceed those to keep", lambda: gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 5, 3, 3, 0, 0, o.ptr)),
+                        ("no such layers", lambda: gpu.kv_evict_device(c.cache, c.seqs, 1, 2, 5, 3, 2, 0, 0, o.ptr)),
+                        ("do not hold what is kept", lambda: gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 17, 3, 2, b.ptr, 1, o.ptr)),
+                        ("no such layer", lambda: gpu.kv_store_device(c.cache, c.seqs, 2, b.ptr, b.ptr))):
+        with pytest.raises(pkg.NativeHipError, match=match) as e:
+            call()
+        assert e.value.code == pkg.ERR_INVALID
+    c.cache.ggml_type = pkg.Q8_0
+    with pytest.raises(pkg.NativeHipError, match="f32 or f16") as e:
+        attn()
+    assert e.value.code == pkg.ERR_UNSUPPORTED
+    hip.device_synchronize()
+    assert np.all(o.to_numpy(np.float32) == 5)
+    assert all(same_bits(x, y) for x, y in zip(c.down(), (c.k, c.v, c.w)))
+
+
+def test_nothing_to_do_is_done(gpu, hip, pkg):
+    """No sequence, no token, no position: the calls succeed."""
+    rng = np.random.default_rng(0)
+    c = Paged(rng, False, 1, 1, 64, 16, [30], weights=True, garbage=0.0).up()
+    none = pkg.KvSeqs(0, 0, 2, 0, 0, n_tokens=0)
+    gpu.kv_store_device(c.cache, none, 0, 0, 0)
+    gpu.attn_device(c.cache, none, 0, 1, 0, 0, 0.125)
+    gpu.kv_evict_device(c.cache, none, 0, 1, 5, 0, 0, 0, 0, 0)
+    c.dl.upload(np.array([0], np.uint32))
+    c.seqs.max_len = 0
+    out = attend(gpu, c, 0, np.ones((1, 2, 64), np.float32), 0.125, weights=True)
+    assert np.all(out == 0)
+    assert all(same_bits(x, y) for x, y in zip(c.down(), (c.k, c.v, c.w)))
