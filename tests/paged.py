@@ -91,7 +91,7 @@ class Paged:
                             size = (np.abs(k[sees]) @ np.abs(qr)).max() * abs(scale)
                             rel = (2 * (self.d + 24) * size + int(sees.sum()) + 80) * 2.0 ** -23
                             tol[row, head] = rel * (pr @ np.abs(v[sees])) + 1e-37
-                        ws[sees] += pr
+                            ws[sees] += pr
                             wt[sees] += (rel + n * group * 2.0 ** -23) * pr + 2.0 ** -120
                 if n:
                     sums[b, h] = (pos, ws, wt)
