@@ -25,6 +25,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 
 #include "attn_rows.inc"
 #include "attn_split.inc"
+#include "attn_chunk.inc"
 #include "attn_weights.inc"
 #include "kv_store.inc"
 #include "kv_evict.inc"
