@@ -30,6 +30,7 @@
 #include <hip/hip_fp16.h>
 
 #include "../../include/native_hip.h"
+#include "../../include/native_hip_attention.h"
 #include "../../include/native_hip_llama.h"
 #include "gguf.h"
 #include "head_step.h"
@@ -1351,6 +1352,20 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
     lnm_session *s = nullptr;
     if (lnm_session_new(model, kv_block, block_ids, n_block_ids, &s) != 0) return 1;
     if (device_decode_create(s, max_positions) != 0) {
+        delete s;
+        *out = nullptr;
+        return 1;
+    }
+    *out = s;
+    return 0;
+}
+
+int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids, size_t max_positions,
+                                 uint32_t kv_type, size_t window, size_t sinks, lnm_session **out) {
+    lnm_session *s = nullptr;
+    if (lnm_session_new(model, kv_block, block_ids, n_block_ids, &s) != 0) return 1;
+    const PagedKv paged{kv_type, window, sinks};
+    if (device_decode_create(s, max_positions, &paged) != 0) {
         delete s;
         *out = nullptr;
         return 1;

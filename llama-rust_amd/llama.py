@@ -169,9 +169,10 @@ class Llama:
         _check(_pkg.load_library().lnm_moe_ffn(self._h, layer, x.shape[0], x.ctypes.data, out.ctypes.data))
         return out
 
-    def session(self, kv_block=16, block_ids=None, device_positions=None):
-        """device_positions: keep the whole decode step on the GPU, with a cache of that many positions."""
-        return Session(self, kv_block, block_ids, device_positions)
+    def session(self, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0):
+        """device_positions: keep the whole decode step on the GPU, with a cache of that many positions; kv_type (F32 or F16): over
+        the paged-cache operators, a token seeing the last `window` positions (0: all) and the first `sinks`."""
+        return Session(self, kv_block, block_ids, device_positions, kv_type, window, sinks)
 
     def batch_session(self, n_sequences, device_positions, kv_block=16):
         """A device session that decodes `n_sequences` sequences together, one token of each per step."""
@@ -220,16 +221,22 @@ class BatchSession:
 
 
 class Session:
-    def __init__(self, model, kv_block=16, block_ids=None, device_positions=None):
+    def __init__(self, model, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0):
         lib = _pkg.load_library()
+        if kv_type is None and (window or sinks):
+            raise LlamaError("a window needs a session with a kv_type")
+        if kv_type is not None and device_positions is None:
+            raise LlamaError("a kv_type needs device_positions")
         self.model = model
         h = C.c_void_p()
         ids = None if block_ids is None else np.ascontiguousarray(block_ids, dtype=np.uint32)
         ids_p, ids_n = (None, 0) if ids is None else (ids.ctypes.data, ids.size)
         if device_positions is None:
             _check(lib.lnm_session_new(model._h, kv_block, ids_p, ids_n, C.byref(h)))
-        else:
+        elif kv_type is None:
             _check(lib.lnm_session_new_device(model._h, kv_block, ids_p, ids_n, device_positions, C.byref(h)))
+        else:
+            _check(lib.lnm_session_new_device_paged(model._h, kv_block, ids_p, ids_n, device_positions, kv_type, window, sinks, C.byref(h)))
         self._h = h
 
     def forward(self, tokens):
