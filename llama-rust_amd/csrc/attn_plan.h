@@ -60,6 +60,15 @@ NH_ATTN_HD bool attn_sees(int32_t p, uint32_t t, uint32_t window, uint32_t sinks
     return window == 0 || (uint32_t)p - t < window || t < sinks;
 }
 
+// The sequence's new tokens that see position t: from .. to.
+struct SeenBy {
+    uint32_t from, to;
+};
+NH_ATTN_HD SeenBy attn_seen_by(const SeqRows &s, uint32_t t, uint32_t window, uint32_t sinks) {
+    const int64_t from = (int64_t)t - s.first_pos, to = from + window, n = s.n;
+    return {(uint32_t)(from < 0 ? 0 : from < n ? from : n), (uint32_t)(window == 0 || t < sinks || to > n ? n : to < 0 ? 0 : to)};
+}
+
 // The tiles of `tp` positions that tokens at first_pos .. last_pos read, the first tokens' and then the window's, none twice.
 struct AttnTiles {
     uint32_t sink_tiles, from, count;
