@@ -40,6 +40,6 @@ struct KvEvictCall {
     uint32_t *new_lens;
 };
 size_t kv_evict_workspace_bytes(const KvEvictCall &c);
-hipError_t launch_kv_evict(hipStream_t stream, const KvEvictCall &c, void *ws);
+hipError_t launch_kv_evict(hipStream_t stream, const KvEvictCall &c, uint32_t cus, void *ws);
 
 }  // namespace nh
