@@ -489,3 +489,140 @@ def test_nothing_to_do_is_done(gpu, hip, pkg):
     out = attend(gpu, c, 0, np.ones((1, 2, 64), np.float32), 0.125, weights=True)
     assert np.all(out == 0)
     assert all(same_bits(x, y) for x, y in zip(c.down(), (c.k, c.v, c.w)))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("block", [16, 7])
+def test_more_sequences_and_heads_than_compute_units(gpu, f16, block):
+    """Sequences of any length among 300, whose units alone are more than one round; every fifth holds nothing, every seventh is long."""
+    rng = np.random.default_rng(block)
+    lens = [0 if i % 5 == 4 else int(rng.integers(200, 400)) if i % 7 == 3 else int(rng.integers(1, 30)) for i in range(300)]
+    c = Paged(rng, f16, 1, 1, 16, block, lens, weights=True).up()
+    q = rng.normal(0, 1, (300, 2, 16)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, 0.25)
+    check(attend(gpu, c, 0, q, 0.25, weights=True), want, tol)
+    w, w_tol = c.weigh(0, sums, 1.0)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert same_bits(after[~held], c.w[~held]) and np.all(np.abs(after[held] - w[held]) <= w_tol[held])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("heads,hkv,d,new,lens,window,sinks", [
+    (20, 1, 64, 1, [1500, 3, 900], 0, 0),      # two tiles of rows of one token
+    (4, 2, 128, 13, [1300, 13, 400], 0, 0),    # 26 rows a key-value head
+    (4, 2, 128, 13, [1300, 13, 400], 300, 20),
+    (8, 2, 64, 80, [1100, 80], 0, 0),          # blocks of rows that share their steps
+    (8, 2, 64, 80, [1100, 80], 500, 3),
+    (4, 1, 200, 40, [700, 41], 0, 0),
+    (2, 1, 128, 300, [900, 310], 0, 0),        # several blocks of rows, the last of them short
+    (2, 1, 128, 300, [900, 310], 128, 64),
+])
+def test_rows_and_positions_are_cut(gpu, f16, heads, hkv, d, new, lens, window, sinks):
+    """Between the smallest and the largest variants, with the weights: tokens of several sequences behind long histories."""
+    rng = np.random.default_rng(new + d)
+    starts = [new * i for i in range(len(lens) + 1)]
+    c = Paged(rng, f16, 1, hkv, d, 16, lens, weights=True).up(starts, max_new=new)
+    q = rng.normal(0, 1, (starts[-1], heads, d)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, d ** -0.5, starts, window, sinks)
+    check(attend(gpu, c, 0, q, np.float32(d ** -0.5), window=window, sinks=sinks, weights=True, decay=0.75), want, tol + 1e-7 * np.abs(want))
+    w, w_tol = c.weigh(0, sums, 0.75)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert same_bits(after[~held], c.w[~held])
+    off = np.abs(after[held] - w[held])
+    assert np.all(off <= w_tol[held] + 2e-7 * w[held]), np.max(off - w_tol[held])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_weights_of_many_rows_beside_what_is_not_finite(gpu, f16, bad):
+    """A key that is infinite or NaN at a late position: the tokens before it and their sums do not know of it."""
+    rng = np.random.default_rng(31)
+    c = Paged(rng, f16, 1, 1, 64, 16, [200], weights=True)
+    c.w[:] = 0
+    c.k[c.tables[0, 150 // 16], 0, 0, 150 % 16, 3] = bad
+    c.up([0, 150], max_new=150)
+    q = rng.normal(0, 1, (150, 1, 64)).astype(np.float32)
+    q[:, 0, 3] = np.abs(q[:, 0, 3]) + 0.5
+    got = attend(gpu, c, 0, q, 0.125, weights=True)
+    after = c.down()[2]
+    # tokens stand at 50 ..: those before 150 are as without the position, those from it see it
+    clean = Paged(np.random.default_rng(31), f16, 1, 1, 64, 16, [200], weights=True)
+    want, tol, _ = clean.attend(0, q, 0.125, [0, 150])
+    check(got[:100], want[:100], tol[:100])
+    if bad == -np.inf:  # a score of minus infinity is a position without weight
+        assert np.all(np.isfinite(got)) and np.all(np.isfinite(after))
+        assert after[c.tables[0, 9], 0, 0, 6] == 0
+        assert abs(after.sum() - 150) < 1e-3
+    else:
+        assert np.all(np.isnan(got[100:]))
+        seen = [after[c.tables[0, t // 16], 0, 0, t % 16] for t in range(200)]
+        assert np.all(np.isnan(seen[:151]))  # a row of NaN gives every position it sees one
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction_of_a_middle_beyond_one_block_of_keys(gpu, hip, in_place):
+    """40000 positions, most weights equal to another's: the earliest of the equal ones stay."""
+    rng = np.random.default_rng(6)
+    lens, keep = [40000, 16500, 17000], 16400
+    c = Paged(rng, True, 1, 1, 8, 64, lens, garbage=0, weights=True, extra_blocks=3 * 257)
+    c.w[:] = rng.integers(0, 50, c.w.shape).astype(np.float32)
+    for t in range(0, 40000, 3):
+        c.w[c.at(0, t)] = np.float32(rng.exponential(30))
+    c.up()
+    dst = c.free[:3 * 257].reshape(3, 257).astype(np.uint32)
+    dd, new = hip.DeviceBuffer.from_numpy(dst), hip.DeviceBuffer(12)
+    gpu.kv_evict_device(c.cache, c.seqs, 0, 1, keep, 4, 100, 0 if in_place else dd.ptr, 0 if in_place else 257, new.ptr)
+    hip.device_synchronize()
+    want_len, k, v, w = c.evict([0], keep, 4, 100, None if in_place else dst)
+    assert new.to_numpy(np.uint32).tolist() == want_len.tolist()
+    for got, want in zip(c.down(), (k, v, w)):
+        assert same_bits(got, want)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("d,hkv,layers", [(8, 1, 1), (40, 3, 2), (104, 1, 1), (128, 2, 1), (256, 1, 1)])
+def test_eviction_in_place_in_strips(gpu, hip, f16, d, hkv, layers):
+    """Rows of any size move forward past the end of a strip of rows; nothing to move at the front, everything behind it."""
+    rng = np.random.default_rng(d)
+    lens = [2600, 1100]
+    c = Paged(rng, f16, layers, hkv, d, 16, lens, garbage=-2.0, weights=True).up()
+    gpu.kv_evict_device(c.cache, c.seqs, 0, layers, 2100, 0, 0, 0, 0, c.dl.ptr)
+    hip.device_synchronize()
+    want_len, k, v, w = c.evict(range(layers), 2100, 0, 0)
+    assert c.dl.to_numpy(np.uint32).tolist() == want_len.tolist()
+    for got, want in zip(c.down(), (k, v, w)):
+        assert same_bits(got, want)
+
+
+def test_two_executors_at_once(pkg, hip):
+    """Calls on streams of two executors, each with its own workspace, none waited for: the results of each alone."""
+    rng = np.random.default_rng(17)
+    made = []
+    for f16, heads, lens in ((True, 8, [3000, 20, 700]), (False, 4, [100, 2500])):
+        g, stream = pkg.HipGemv(0), hip.Stream()
+        c = Paged(rng, f16, 1, 2, 64, 16, lens, weights=True, garbage=0).up()
+        q = rng.normal(0, 1, (len(lens), heads, 64)).astype(np.float32)
+        dq, outs = hip.DeviceBuffer.from_numpy(q), [hip.DeviceBuffer(q.nbytes) for _ in range(21)]
+        made.append((g, stream, c, heads, dq, outs))
+    hip.device_synchronize()
+
+    def run(i, k):
+        g, stream, c, heads, dq, outs = made[i]
+        g.attn_device(c.cache, c.seqs, 0, heads, dq.ptr, outs[k].ptr, 0.125, weights=True, decay=0.5, stream=stream.ptr)
+
+    for i in range(2):
+        run(i, 20)
+        hip.device_synchronize()
+    for k in range(20):
+        for i in range(2):
+            run(i, k)
+    hip.device_synchronize()
+    for g, stream, c, heads, dq, outs in made:
+        want = outs[20].to_numpy(np.float32)
+        assert np.all(np.isfinite(want))
+        for o in outs[:20]:
+            assert np.array_equal(o.to_numpy(np.float32), want)
+        stream.destroy()
+        g.close()
