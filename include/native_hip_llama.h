@@ -82,9 +82,9 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
  * each head one workgroup), a prompt's runs on the matrix cores, the block table may be of any length, and with window > 0 a token
  * sees the last `window` positions and the first `sinks` (every position stays in the cache).  Without a window and with f32,
  * results are the session above's but for the order of sums.  Four layers of 4096 columns, 32 heads of 128 over 8 (that
- * session, f32, f16): behind 128 positions a step takes 214, 235, 234 us (three launches a layer in place of one), behind 2048
- * 304, 260, 251, behind 16384 1246, 361, 303 and with a window of 1024 244; a prompt of 2048 18.8, 12.1, 11.3 ms, of 16384 1410,
- * 145, 99 ms.  Heads of a multiple of 8, at most 256. */
+ * session, f32, f16): behind 128 positions a step takes 200, 222, 219 us (three launches a layer in place of one), behind 2048
+ * 287, 240, 231, behind 16384 1223, 344, 293 and with a window of 1024 233; a prompt of 2048 18.0, 11.9, 11.1 ms, of 16384 1400,
+ * 134, 91 ms.  Heads of a multiple of 8, at most 256. */
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,
                                  size_t max_positions, uint32_t kv_type, size_t window, size_t sinks, lnm_session **out);
 /* A device session for `n_sequences` (at most 128) independent sequences of up to `max_positions` each, decoded
