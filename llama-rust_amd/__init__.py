@@ -158,6 +158,7 @@ def load_library():
         "lnm_session_new_device": (C.c_int, [vp, sz, vp, sz, sz, pvp]),
         "lnm_session_new_device_paged": (C.c_int, [vp, sz, vp, sz, sz, u32, sz, sz, pvp]),
         "lnm_session_new_device_batch": (C.c_int, [vp, sz, sz, sz, pvp]),
+        "lnm_session_new_device_batch_paged": (C.c_int, [vp, sz, sz, sz, u32, sz, sz, pvp]),
         "lnm_batch_generate_greedy": (C.c_int, [vp, vp, vp, sz, vp, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
         "lnm_session_free": (None, [vp]),
         "lnh_act_create": (C.c_int, [vp, C.c_uint32, sz, sz, vp]),

@@ -1387,6 +1387,20 @@ int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_seq
     return 0;
 }
 
+int lnm_session_new_device_batch_paged(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions, uint32_t kv_type, size_t window,
+                                       size_t sinks, lnm_session **out) {
+    lnm_session *s = nullptr;
+    if (lnm_session_new(model, kv_block, nullptr, 0, &s) != 0) return 1;
+    const PagedKv paged{kv_type, window, sinks};
+    if (device_batch_create(s, n_sequences, max_positions, &paged) != 0) {
+        delete s;
+        *out = nullptr;
+        return 1;
+    }
+    *out = s;
+    return 0;
+}
+
 int lnm_batch_generate_greedy(lnm_session *session, const uint32_t *prompts, const size_t *prompt_lens, size_t n_new,
                               uint32_t *out, double *prefill_seconds, double *decode_seconds) {
     if (!session || !prompts || !prompt_lens || !out) return fail("null argument");

@@ -174,9 +174,9 @@ class Llama:
         the paged-cache operators, a token seeing the last `window` positions (0: all) and the first `sinks`."""
         return Session(self, kv_block, block_ids, device_positions, kv_type, window, sinks)
 
-    def batch_session(self, n_sequences, device_positions, kv_block=16):
-        """A device session that decodes `n_sequences` sequences together, one token of each per step."""
-        return BatchSession(self, n_sequences, device_positions, kv_block)
+    def batch_session(self, n_sequences, device_positions, kv_block=16, kv_type=None, window=0, sinks=0):
+        """A device session that decodes `n_sequences` sequences together, one token of each per step; kv_type, window, sinks: as in session()."""
+        return BatchSession(self, n_sequences, device_positions, kv_block, kv_type, window, sinks)
 
     def close(self):
         if self._h:
@@ -191,10 +191,16 @@ class Llama:
 
 
 class BatchSession:
-    def __init__(self, model, n_sequences, device_positions, kv_block=16):
+    def __init__(self, model, n_sequences, device_positions, kv_block=16, kv_type=None, window=0, sinks=0):
+        lib = _pkg.load_library()
+        if kv_type is None and (window or sinks):
+            raise LlamaError("a window needs a session with a kv_type")
         self.model, self.n_sequences = model, n_sequences
         h = C.c_void_p()
-        _check(_pkg.load_library().lnm_session_new_device_batch(model._h, kv_block, n_sequences, device_positions, C.byref(h)))
+        if kv_type is None:
+            _check(lib.lnm_session_new_device_batch(model._h, kv_block, n_sequences, device_positions, C.byref(h)))
+        else:
+            _check(lib.lnm_session_new_device_batch_paged(model._h, kv_block, n_sequences, device_positions, kv_type, window, sinks, C.byref(h)))
         self._h = h
 
     def generate_greedy(self, prompts, n_new):

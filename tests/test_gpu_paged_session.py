@@ -172,3 +172,52 @@ def test_refusals(pkg, llama, model, tmp_path):
     assert len(narrow.session(device_positions=16).forward([1, 2])) == 256
     with pytest.raises(llama.LlamaError, match="multiple of 8"):
         narrow.session(device_positions=16, kv_type=pkg.F32)
+
+
+LENGTHS = [40, 1, 1, 300, 7, 2, 513, 1, 90, 33]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 3)])
+def test_a_batch_equals_its_sequences_alone(pkg, llama, model, half, window, sinks):
+    """Prompts of one token to more than a chunk, chunks that end one prompt and begin another: the tokens that the batch picks are those
+    whose logits are largest in the forward pass over what it picked before, to the sessions' bound."""
+    m, path = model
+    rng = np.random.default_rng(14)
+    prompts = [rng.integers(0, 512, n).tolist() for n in LENGTHS]
+    kind = pkg.F16 if half else pkg.F32
+    batch = m.batch_session(len(prompts), 530, kv_block=9, kv_type=kind, window=window, sinks=sinks)
+    got, _, _ = batch.generate_greedy(prompts, 12)
+    again, _, _ = batch.generate_greedy(prompts[::-1], 12)  # other lengths through the same graph
+    for prompt, tokens, other in zip(prompts, got, again[::-1]):
+        for picked in (tokens, other):
+            whole = prompt + picked.tolist()
+            want = forward(llama, path, m.hparams, whole, window, sinks, half)
+            tol = 2e-4 * np.abs(want).max()
+            if half:
+                tol += np.abs(want - forward(llama, path, m.hparams, whole, window, sinks)).max() / 4
+            for i, t in enumerate(picked):
+                logits = want[len(prompt) - 1 + i]
+                assert logits[t] >= logits.max() - 2 * tol, (len(prompt), i)
+
+
+def test_a_batch_of_the_largest_size(pkg, llama, model):
+    m, _ = model
+    prompts = [[int(x) for x in np.random.default_rng(i).integers(0, 512, 1 + i % 5)] for i in range(128)]
+    beside, _, _ = m.batch_session(128, 64).generate_greedy(prompts, 8)
+    here, _, _ = m.batch_session(128, 64, kv_type=pkg.F32).generate_greedy(prompts, 8)
+    assert np.array_equal(here, beside)
+
+
+def test_batch_refusals(pkg, llama, model):
+    m, _ = model
+    with pytest.raises(llama.LlamaError, match="f32 or f16"):
+        m.batch_session(2, 16, kv_type=pkg.Q8_0)
+    with pytest.raises(llama.LlamaError, match="sinks without one"):
+        m.batch_session(2, 16, kv_type=pkg.F16, sinks=1)
+    with pytest.raises(llama.LlamaError, match="kv_type"):
+        m.batch_session(2, 16, window=1)
+    s = m.batch_session(2, 16, kv_type=pkg.F16)
+    with pytest.raises(llama.LlamaError, match="outgrew"):
+        s.generate_greedy([[1] * 10, [2]], 8)
+    assert s.generate_greedy([[1] * 9, [2]], 8)[0].shape == (2, 8)
