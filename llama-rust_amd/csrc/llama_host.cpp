@@ -32,6 +32,7 @@
 #include "../../include/native_hip.h"
 #include "../../include/native_hip_attention.h"
 #include "../../include/native_hip_llama.h"
+#include "attn_plan.h"
 #include "gguf.h"
 #include "head_step.h"
 #include "host_pool.h"
@@ -1263,6 +1264,25 @@ void random_rows(uint32_t type, size_t n_cols, size_t n_rows, float sigma, uint6
 
 #include "llama_device.inc"
 
+namespace {
+
+// A session that create(session) makes one of the device's; no exception passes.
+template <typename Create>
+int paged_session(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids, lnm_session **out, Create &&create) try {
+    if (!out) return fail("null argument");
+    *out = nullptr;
+    lnm_session *made = nullptr;
+    if (lnm_session_new(model, kv_block, block_ids, n_block_ids, &made) != 0) return 1;
+    std::unique_ptr<lnm_session> s(made);
+    if (create(s.get()) != 0) return 1;
+    *out = s.release();
+    return 0;
+} catch (const std::exception &e) {
+    return fail(std::string("paged session: ") + e.what());
+}
+
+}  // namespace
+
 // ------------------------------------------------------------------ C ABI
 
 extern "C" {
@@ -1362,16 +1382,10 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
 
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids, size_t max_positions,
                                  uint32_t kv_type, size_t window, size_t sinks, lnm_session **out) {
-    lnm_session *s = nullptr;
-    if (lnm_session_new(model, kv_block, block_ids, n_block_ids, &s) != 0) return 1;
-    const PagedKv paged{kv_type, window, sinks};
-    if (device_decode_create(s, max_positions, &paged) != 0) {
-        delete s;
-        *out = nullptr;
-        return 1;
-    }
-    *out = s;
-    return 0;
+    return paged_session(model, kv_block, block_ids, n_block_ids, out, [&](lnm_session *s) {
+        const PagedKv paged{kv_type, window, sinks};
+        return device_decode_create(s, max_positions, &paged);
+    });
 }
 
 int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions,
@@ -1389,16 +1403,10 @@ int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_seq
 
 int lnm_session_new_device_batch_paged(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions, uint32_t kv_type, size_t window,
                                        size_t sinks, lnm_session **out) {
-    lnm_session *s = nullptr;
-    if (lnm_session_new(model, kv_block, nullptr, 0, &s) != 0) return 1;
-    const PagedKv paged{kv_type, window, sinks};
-    if (device_batch_create(s, n_sequences, max_positions, &paged) != 0) {
-        delete s;
-        *out = nullptr;
-        return 1;
-    }
-    *out = s;
-    return 0;
+    return paged_session(model, kv_block, nullptr, 0, out, [&](lnm_session *s) {
+        const PagedKv paged{kv_type, window, sinks};
+        return device_batch_create(s, n_sequences, max_positions, &paged);
+    });
 }
 
 int lnm_batch_generate_greedy(lnm_session *session, const uint32_t *prompts, const size_t *prompt_lens, size_t n_new,
