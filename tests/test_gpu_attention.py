@@ -626,3 +626,25 @@ def test_two_executors_at_once(pkg, hip):
             assert np.array_equal(o.to_numpy(np.float32), want)
         stream.destroy()
         g.close()
+
+
+def test_calls_larger_than_a_launch_are_refused(gpu, hip, pkg):
+    """Sizes whose products pass 32 and 64 bits: refused by their numbers, with nothing launched."""
+    rng = np.random.default_rng(0)
+    c = Paged(rng, True, 1, 1, 64, 16, [20, 20], weights=True, garbage=0).up([0, 1, 2])
+    q, out = hip.DeviceBuffer(1 << 16), hip.DeviceBuffer(1 << 16)
+    out.fill_byte(0x11)
+    hip.device_synchronize()
+    for n_seqs, n_tokens, max_new, heads in ((1 << 23, 1 << 20, 1, 1), ((1 << 31) - 4096, 64, 64, 1), ((1 << 31) - 4096, (1 << 31) - 4096, (1 << 31) // 65536 - 1, 65536),
+                                             (1, (1 << 31) - 4096, (1 << 31) - 4096, 1)):
+        seqs = pkg.KvSeqs(n_seqs, c.dt.ptr, c.stride, c.dl.ptr, 20, c.ds.ptr, n_tokens, max_new)
+        for weights in (False, True):
+            with pytest.raises(pkg.NativeHipError, match="larger than one launch"):
+                gpu.attn_device(c.cache, seqs, 0, heads, q.ptr, out.ptr, 0.125, weights=weights)
+    many = pkg.KvSeqs(1 << 23, c.dt.ptr, c.stride, c.dl.ptr, 20, c.ds.ptr, 64, 1)
+    with pytest.raises(pkg.NativeHipError, match="larger than one launch"):
+        gpu.kv_store_device(c.cache, many, 0, q.ptr, q.ptr)
+    with pytest.raises(pkg.NativeHipError, match="larger than one launch"):
+        gpu.kv_evict_device(c.cache, many, 0, 1, 4, 0, 0, 0, 0, c.dl.ptr)
+    hip.device_synchronize()
+    assert np.all(out.to_numpy(np.uint8) == 0x11) and np.array_equal(c.dl.to_numpy(np.uint32), c.lens)
