@@ -59,7 +59,7 @@ int lnh_kv_store_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_
                         const float *device_k, size_t k_stride, const float *device_v, size_t v_stride, void *stream);
 
 /* out = softmax(scale q K^T) V for every new token and each of n_head query heads (a multiple of n_head_kv; query
- * head h reads key-value head h * n_head_kv / n_head), over `layer` of the cache: the new tokens' own rows have to be
+ * head h reads key-value head h * n_head_kv / n_head; 0 < scale <= 2^127), over `layer` of the cache: the new tokens' own rows have to be
  * stored before.  The token at position p sees position t where t <= p and, with window > 0, p - t < window or
  * t < sinks (sinks without a window: LNH_ERR_INVALID).  Rows of q and out are n_head * head_dim floats, strides in
  * floats.  A token that sees nothing gets zeros; so does one whose every score is -infinity.  What lies in positions

@@ -168,6 +168,8 @@ inline AttnCheck check_attn(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t 
     if (n_head > 65536) return {LNH_ERR_INVALID, "more than 65536 query heads"};
     if (s->max_new > ATTN_MAX_POSITIONS / (n_head / c->n_head_kv)) return {LNH_ERR_INVALID, "tokens times query heads exceed 31 bits"};
     if (!std::isfinite(scale) || !std::isfinite(decay)) return {LNH_ERR_INVALID, "scale and decay must be finite"};
+    // places that a row does not see are given minus infinity before the multiplication; 2^127 leaves room for log2(e)
+    if (scale <= 0.f || scale > 0x1p127f) return {LNH_ERR_INVALID, "scale must be positive, at most 2^127"};
     if (window > ATTN_MAX_POSITIONS || sinks > ATTN_MAX_POSITIONS) return {LNH_ERR_INVALID, "window or sinks exceed 31 bits"};
     if (window == 0 && sinks != 0) return {LNH_ERR_INVALID, "first tokens stay visible beside a window: sinks without one"};
     if (s->n_seqs == 0 || s->n_tokens == 0 || s->max_new == 0) return {LNH_OK, nullptr};

@@ -165,6 +165,8 @@ static void refusals() {
     CHECK(call(0, 4, nullptr, 256, buf, 256, 1.f, 0, 0, 1.f) == LNH_ERR_INVALID);
     CHECK(call(0, 4, buf, 256, buf + 48, 256, std::numeric_limits<float>::quiet_NaN(), 0, 0, 1.f) == LNH_ERR_INVALID);
     CHECK(call(0, 4, buf, 256, buf + 48, 256, 1.f, 0, 0, std::numeric_limits<float>::infinity()) == LNH_ERR_INVALID);
+    for (const float scale : {0.f, -0.f, -0.125f, std::numeric_limits<float>::max()}) CHECK(call(0, 4, buf, 256, buf + 48, 256, scale, 0, 0, 1.f) == LNH_ERR_INVALID);
+    for (const float scale : {1e-30f, 0x1p127f}) CHECK(call(0, 4, buf, 256, buf + 48, 256, scale, 0, 0, 1.f) == LNH_OK);
     CHECK(call(0, 4, buf, 256, buf + 48, 256, 1.f, 0, 4, 1.f) == LNH_ERR_INVALID);
     CHECK(call(0, 4, buf, 256, buf + 48, 256, 1.f, (size_t)1 << 31, 4, 1.f) == LNH_ERR_INVALID);
     CHECK(nh::check_kv_store(&good, &seqs, 0, buf, 256, buf, 256).code == LNH_OK);
@@ -190,7 +192,24 @@ static void refusals() {
     CHECK(evict(0, 1, 500, 4, 4, idx + 32, 7, idx) == LNH_OK);  // never more than max_len
 }
 
+// The tokens that see a position, by the position.
+static void seen_by() {
+    for (const uint32_t n : {0u, 1u, 7u, 40u})
+        for (const int32_t first : {-41, -5, 0, 3, 100})
+            for (const uint32_t window : {0u, 1u, 6u, 30u, 0x7fffefffu})
+                for (const uint32_t sinks : {0u, 2u, 50u, 0x7fffefffu}) {
+                    if (window == 0 && sinks != 0) continue;
+                    const nh::SeqRows s{0, n, first, first + (int32_t)n > 0 ? (uint32_t)(first + (int32_t)n) : 0u};
+                    for (uint32_t t = 0; t < 160; t++) {
+                        const nh::SeenBy by = nh::attn_seen_by(s, t, window, sinks);
+                        CHECK(by.from <= n && by.to <= n);
+                        for (uint32_t i = 0; i < n; i++) CHECK(nh::attn_sees(first + (int32_t)i, t, window, sinks) == (by.from <= i && i < by.to));
+                    }
+                }
+}
+
 int main() {
+    seen_by();
     division();
     tiles();
     sight();

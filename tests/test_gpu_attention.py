@@ -648,3 +648,33 @@ def test_calls_larger_than_a_launch_are_refused(gpu, hip, pkg):
         gpu.kv_evict_device(c.cache, many, 0, 1, 4, 0, 0, 0, 0, c.dl.ptr)
     hip.device_synchronize()
     assert np.all(out.to_numpy(np.uint8) == 0x11) and np.array_equal(c.dl.to_numpy(np.uint32), c.lens)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("heads,hkv,d,block,window,sinks", [(4, 4, 128, 16, 0, 0), (8, 1, 256, 20, 0, 0), (10, 2, 96, 16, 40, 2), (40, 2, 40, 7, 0, 0), (9, 1, 192, 64, 33, 0),
+                                                            (2, 1, 8, 3, 0, 0), (6, 3, 136, 16, 0, 0)])
+def test_weights_and_long_shares_in_other_layouts(gpu, f16, heads, hkv, d, block, window, sinks):
+    """A prompt, a remainder behind a long history (many shares) and one token beside them, with the weights."""
+    rng = np.random.default_rng(d + block)
+    starts, lens = [0, 70, 75, 76], [90, 1500, 33]
+    c = Paged(rng, f16, 1, hkv, d, block, lens, weights=True).up(starts, max_new=70)
+    q = rng.normal(0, 1, (76, heads, d)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, d ** -0.5, starts, window, sinks)
+    check(attend(gpu, c, 0, q, np.float32(d ** -0.5), window=window, sinks=sinks, weights=True, decay=1.0), want, tol + 1e-7 * np.abs(want))
+    w, w_tol = c.weigh(0, sums, 1.0)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert same_bits(after[~held], c.w[~held])
+    off = np.abs(after[held] - w[held])
+    assert np.all(off <= w_tol[held] + 2e-7 * w[held]), np.max(off - w_tol[held])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("tokens", [1, 5, 16, 40])
+def test_few_tokens_behind_a_long_history(gpu, f16, tokens):
+    """Of one sequence: as many shares as the chip holds, joined side by side."""
+    rng = np.random.default_rng(tokens)
+    c = Paged(rng, f16, 1, 1, 128, 16, [9000]).up([0, tokens], max_new=tokens)
+    q = rng.normal(0, 1, (tokens, 4, 128)).astype(np.float32)
+    want, tol, _ = c.attend(0, q, 128 ** -0.5, [0, tokens])
+    check(attend(gpu, c, 0, q, np.float32(128 ** -0.5)), want, tol + 1e-7 * np.abs(want))
