@@ -82,9 +82,9 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
  * each head one workgroup), a prompt's runs on the matrix cores, the block table may be of any length, and with window > 0 a token
  * sees the last `window` positions and the first `sinks` (every position stays in the cache).  Without a window and with f32,
  * results are the session above's but for the order of sums.  Four layers of 4096 columns, 32 heads of 128 over 8 (that
- * session, f32, f16): behind 128 positions a step takes 200, 222, 219 us (three launches a layer in place of one), behind 2048
- * 287, 240, 231, behind 16384 1223, 344, 293 and with a window of 1024 233; a prompt of 2048 18.0, 11.9, 11.1 ms, of 16384 1400,
- * 134, 91 ms.  Heads of a multiple of 8, at most 256. */
+ * session, f32, f16): behind 128 positions a step takes 198, 219, 216 us (three launches a layer in place of one), behind 2048
+ * 284, 238, 228, behind 16384 1222, 344, 290 and with a window of 1024 234; a prompt of 2048 17.9, 11.5, 11.0 ms, of 16384 1380,
+ * 133, 91 ms.  Heads of a multiple of 8, at most 256. */
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,
                                  size_t max_positions, uint32_t kv_type, size_t window, size_t sinks, lnm_session **out);
 /* A device session for `n_sequences` (at most 128) independent sequences of up to `max_positions` each, decoded
@@ -97,8 +97,8 @@ int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_seq
                                  lnm_session **out);
 /* The batch session over the paged-cache operators, like lnm_session_new_device_paged: the steps' attention as one call over the cut
  * of all sequences, a prompt chunk that ends one prompt and begins the next as rows of several sequences.  The four layers above,
- * 32 sequences (batch session, f32, f16): a step behind 64 positions 532, 552, 543 us, behind 2000 924, 949, 758 and with a window
- * of 256 583; the prompts of 2000 tokens 539, 359, 325 ms. */
+ * 32 sequences (batch session, f32, f16): a step behind 64 positions 507, 531, 515 us, behind 2000 904, 939, 739 and with a window
+ * of 256 559; the prompts of 2000 tokens 531, 346, 315 ms. */
 int lnm_session_new_device_batch_paged(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions,
                                        uint32_t kv_type, size_t window, size_t sinks, lnm_session **out);
 /* Greedy decode of all sequences from scratch: `prompts` holds the prompts one after the other, prompt_lens[b]
