@@ -84,9 +84,18 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
  * results are the session above's but for the order of sums.  Four layers of 4096 columns, 32 heads of 128 over 8 (that
  * session, f32, f16): behind 128 positions a step takes 198, 219, 216 us (three launches a layer in place of one), behind 2048
  * 284, 238, 228, behind 16384 1222, 344, 290 and with a window of 1024 234; a prompt of 2048 17.9, 11.5, 11.0 ms, of 16384 1380,
- * 133, 91 ms.  Heads of a multiple of 8, at most 256. */
+ * 133, 91 ms.  Heads of a multiple of 8, at most 256.
+ * cache_positions (0: max_positions) bounds what the cache holds at a time.  weights != 0 (without a window): every layer and K/V head
+ * sums the softmax weight each cached position has been given, for lnm_session_evict. */
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,
-                                 size_t max_positions, uint32_t kv_type, size_t window, size_t sinks, lnm_session **out);
+                                 size_t max_positions, uint32_t kv_type, size_t window, size_t sinks, size_t cache_positions,
+                                 int weights, lnm_session **out);
+/* The cache of a paged session with weights cut to `keep` positions, if it holds more: the first `first` of them, the last `recent`
+ * and of those between the ones of the largest weight, for every layer and K/V head (lnh_kv_evict_device).  Later tokens see
+ * what stays; keys keep the rotation of their own position and positions go on counting, up to max_positions.  *cached
+ * (may be NULL): positions the cache holds now.  lnm_prompt reuses such a session's cache for a prompt that goes on where it is, and starts
+ * anew for any other. */
+int lnm_session_evict(lnm_session *session, size_t keep, size_t first, size_t recent, size_t *cached);
 /* A device session for `n_sequences` (at most 128) independent sequences of up to `max_positions` each, decoded
  * together: every step processes one token of every sequence, the weight products as one multi-token product
  * each (the continuous-batching shape of langtax/src/engine.rs:1423-1510, where M = the number of running

@@ -1381,11 +1381,18 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
 }
 
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids, size_t max_positions,
-                                 uint32_t kv_type, size_t window, size_t sinks, lnm_session **out) {
+                                 uint32_t kv_type, size_t window, size_t sinks, size_t cache_positions, int weights, lnm_session **out) {
     return paged_session(model, kv_block, block_ids, n_block_ids, out, [&](lnm_session *s) {
-        const PagedKv paged{kv_type, window, sinks};
+        const PagedKv paged{kv_type, window, sinks, cache_positions, weights != 0};
         return device_decode_create(s, max_positions, &paged);
     });
+}
+
+int lnm_session_evict(lnm_session *session, size_t keep, size_t first, size_t recent, size_t *cached) try {
+    if (!session) return fail("null argument");
+    return device_evict(session, keep, first, recent, cached);
+} catch (const std::exception &e) {
+    return fail(std::string("eviction: ") + e.what());
 }
 
 int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions,
@@ -1404,7 +1411,7 @@ int lnm_session_new_device_batch(lnm_model *model, size_t kv_block, size_t n_seq
 int lnm_session_new_device_batch_paged(lnm_model *model, size_t kv_block, size_t n_sequences, size_t max_positions, uint32_t kv_type, size_t window,
                                        size_t sinks, lnm_session **out) {
     return paged_session(model, kv_block, nullptr, 0, out, [&](lnm_session *s) {
-        const PagedKv paged{kv_type, window, sinks};
+        const PagedKv paged{kv_type, window, sinks, 0, false};
         return device_batch_create(s, n_sequences, max_positions, &paged);
     });
 }
@@ -1435,6 +1442,11 @@ int lnm_prompt(lnm_session *session, const uint32_t *tokens, size_t n, float *lo
     if (session->ids.size() == session->past)  // ids that do not cover the cache are no basis for reuse
         while (lcp < session->ids.size() && lcp < n && session->ids[lcp] == tokens[lcp]) lcp++;
     if (prefix_hit) *prefix_hit = lcp;
+    if (session->dev && device_dropped(session) != 0 && (lcp < session->past || lcp == n)) {  // what an eviction left is no prefix: from the start
+        if (device_restart(session) != 0) return 1;
+        lcp = 0;
+        if (prefix_hit) *prefix_hit = 0;
+    }
     if (lcp == n) lcp = n - 1;  // a full hit recomputes the last token: the logits returned are that token's
     // positions 0 .. lcp-1 stay as they are; everything after them is written again as the sequence grows
     session->past = lcp;

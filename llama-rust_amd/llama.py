@@ -169,10 +169,11 @@ class Llama:
         _check(_pkg.load_library().lnm_moe_ffn(self._h, layer, x.shape[0], x.ctypes.data, out.ctypes.data))
         return out
 
-    def session(self, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0):
+    def session(self, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0, cache_positions=0, weights=False):
         """device_positions: keep the whole decode step on the GPU, with a cache of that many positions; kv_type (F32 or F16): over
-        the paged-cache operators, a token seeing the last `window` positions (0: all) and the first `sinks`."""
-        return Session(self, kv_block, block_ids, device_positions, kv_type, window, sinks)
+        the paged-cache operators, a token seeing the last `window` positions (0: all) and the first `sinks`; cache_positions: a
+        cache of fewer positions than the session has; weights: kept for evict()."""
+        return Session(self, kv_block, block_ids, device_positions, kv_type, window, sinks, cache_positions, weights)
 
     def batch_session(self, n_sequences, device_positions, kv_block=16, kv_type=None, window=0, sinks=0):
         """A device session that decodes `n_sequences` sequences together, one token of each per step; kv_type, window, sinks: as in session()."""
@@ -227,10 +228,10 @@ class BatchSession:
 
 
 class Session:
-    def __init__(self, model, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0):
+    def __init__(self, model, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0, cache_positions=0, weights=False):
         lib = _pkg.load_library()
-        if kv_type is None and (window or sinks):
-            raise LlamaError("a window needs a session with a kv_type")
+        if kv_type is None and (window or sinks or cache_positions or weights):
+            raise LlamaError("a window, cache_positions and weights need a session with a kv_type")
         if kv_type is not None and device_positions is None:
             raise LlamaError("a kv_type needs device_positions")
         self.model = model
@@ -242,8 +243,15 @@ class Session:
         elif kv_type is None:
             _check(lib.lnm_session_new_device(model._h, kv_block, ids_p, ids_n, device_positions, C.byref(h)))
         else:
-            _check(lib.lnm_session_new_device_paged(model._h, kv_block, ids_p, ids_n, device_positions, kv_type, window, sinks, C.byref(h)))
+            _check(lib.lnm_session_new_device_paged(model._h, kv_block, ids_p, ids_n, device_positions, kv_type, window, sinks,
+                                                    cache_positions, int(weights), C.byref(h)))
         self._h = h
+
+    def evict(self, keep, first=0, recent=0):
+        """Positions the cache holds afterwards: it is cut to `keep` of them, the first, the last and the heaviest between."""
+        cached = C.c_size_t()
+        _check(_pkg.load_library().lnm_session_evict(self._h, keep, first, recent, C.byref(cached)))
+        return cached.value
 
     def forward(self, tokens):
         """Logits of the last of `tokens`, run as one batch after everything seen so far."""

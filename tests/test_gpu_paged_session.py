@@ -20,9 +20,10 @@ def llama(pkg):
     return importlib.import_module("llama-rust_amd.llama")
 
 
-def forward(llama, path, hp, tokens, window=0, sinks=0, half=False):
+def forward(llama, path, hp, tokens, window=0, sinks=0, half=False, evict=None, gaps=None):
     """Logits of every position in float64 (langtax/src/decode.rs:2710-3099), a token seeing a window and the first tokens, K and V
-    rounded to f16 where they are kept so."""
+    rounded to f16 where they are kept so.  evict (behind, keep, first, recent): after `behind` tokens every layer and K/V head keeps
+    those positions; gaps gets how far the lightest weight that stays and the heaviest that goes are apart, relative."""
     blob = np.fromfile(path, dtype=np.uint8)
     by = {t[0]: t for t in llama.gguf_tensors(blob)}
 
@@ -54,10 +55,26 @@ def forward(llama, path, hp, tokens, window=0, sinks=0, half=False):
         k = kept(rotated((h @ mat(b + "attn_k.weight").T).reshape(n, hp.n_head_kv, hd)))
         v = kept((h @ mat(b + "attn_v.weight").T).reshape(n, hp.n_head_kv, hd))
         att = np.empty((n, hp.n_head, hd))
-        for head in range(hp.n_head):
-            s = np.where(sees, q[:, head] @ k[:, head // group].T / np.sqrt(hd), -np.inf)
-            e = np.exp(s - s.max(axis=1, keepdims=True))
-            att[:, head] = e / e.sum(axis=1, keepdims=True) @ v[:, head // group]
+        for hkv in range(hp.n_head_kv):
+            scores = [q[:, head] @ k[:, hkv].T / np.sqrt(hd) for head in range(hkv * group, (hkv + 1) * group)]
+
+            def softmax(s, sees):
+                e = np.exp(np.where(sees, s, -np.inf) - np.where(sees, s, -np.inf).max(axis=1, keepdims=True))
+                return e / e.sum(axis=1, keepdims=True)
+            stays = sees
+            if evict is not None and evict[0] > evict[1]:
+                behind, keep, first, recent = evict
+                weight = sum(softmax(s, sees)[:behind, :behind].sum(axis=0) for s in scores)
+                middle = np.arange(first, behind - recent)
+                order = middle[np.argsort(-weight[middle], kind="stable")]
+                left, gone = order[:keep - first - recent], order[keep - first - recent:]
+                if gaps is not None and len(left) and len(gone):
+                    gaps.append(weight[left[-1]] / weight[gone[0]] - 1)
+                dropped = np.zeros(n, bool)
+                dropped[gone] = True
+                stays = sees & ~(dropped[None, :] & (p >= behind))
+            for i, s in enumerate(scores):
+                att[:, hkv * group + i] = softmax(s, stays) @ v[:, hkv]
         x = x + att.reshape(n, -1) @ mat(b + "attn_output.weight").T
         h = norm(x, b + "ffn_norm.weight")
         g = h @ mat(b + "ffn_gate.weight").T
@@ -221,3 +238,94 @@ def test_batch_refusals(pkg, llama, model):
     with pytest.raises(llama.LlamaError, match="outgrew"):
         s.generate_greedy([[1] * 10, [2]], 8)
     assert s.generate_greedy([[1] * 9, [2]], 8)[0].shape == (2, 8)
+
+
+def test_an_evicted_cache_goes_on(pkg, llama, model):
+    """A prompt, some steps, an eviction, a prompt's remainder and steps again, against the forward pass in which later tokens do not
+    see what each layer and head dropped.  What stays is decided by weights that lie apart by far more than their errors (the
+    attention's bound, 2^-23 times a few hundred)."""
+    m, path = model
+    tokens = np.random.default_rng(21).integers(0, 512, 140).tolist()
+    behind, keep, first, recent = 90, 60, 4, 20
+    gaps = []
+    want = forward(llama, path, m.hparams, tokens, evict=(behind, keep, first, recent), gaps=gaps)
+    plain = forward(llama, path, m.hparams, tokens)
+    assert min(gaps) > 1e-4
+    tol = 2e-4 * np.abs(want).max()
+    assert np.abs(want - plain)[behind:].max() > 4 * tol  # the eviction shows
+    s = m.session(kv_block=7, device_positions=140, kv_type=pkg.F32, cache_positions=110, weights=True)
+    assert np.abs(s.forward(tokens[:80]) - want[79]).max() <= tol
+    for i in range(80, behind):
+        assert np.abs(s.forward([tokens[i]]) - want[i]).max() <= tol
+    assert s.evict(200) == behind  # nothing to do
+    assert s.evict(keep, first, recent) == keep
+    done = behind
+    for upto in [91, 92, 120] + list(range(121, 141)):
+        got = s.forward(tokens[done:upto])
+        assert np.abs(got - want[upto - 1]).max() <= tol, upto
+        done = upto
+    with pytest.raises(llama.LlamaError, match="outgrew"):
+        s.forward([1])
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_more_tokens_than_the_cache_holds(pkg, llama, model, half):
+    """Evictions let a sequence pass the cache's size; a prompt that does not go on where it is starts anew, one that does goes on."""
+    m, _ = model
+    kind = pkg.F16 if half else pkg.F32
+    s = m.session(device_positions=400, kv_type=kind, cache_positions=64, weights=True)
+    prompt = np.random.default_rng(22).integers(0, 512, 40).tolist()
+    out = []
+    s.prompt(prompt)
+    last = prompt[-1]
+    for _ in range(40):
+        tokens, _, _ = s.generate_greedy([last], 9)
+        out += tokens.tolist()
+        last = out[-1]
+        assert s.evict(48, 4, 24) == 48
+    assert len(out) == 360 and all(0 <= t < 512 for t in out)
+    with pytest.raises(llama.LlamaError, match="positions"):
+        s.forward([1])
+    fresh, hit = s.prompt(prompt)
+    assert hit == 0
+    want, _ = m.session(device_positions=400, kv_type=kind, cache_positions=64, weights=True).prompt(prompt)
+    assert np.array_equal(fresh, want)
+    s.evict(32, 4, 4)
+    more, hit = s.prompt(prompt + [5, 6, 7])
+    assert hit == 40 and np.all(np.isfinite(more))
+    assert s.evict(64) == 35
+    with pytest.raises(llama.LlamaError, match="cache"):
+        s.forward([1] * 30)
+    assert s.evict(0) == 0
+    assert np.all(np.isfinite(s.forward([1, 2, 3])))
+
+
+def test_weights_leave_the_results_as_they_are(pkg, llama, model):
+    m, _ = model
+    tokens = np.random.default_rng(23).integers(0, 512, 300).tolist()
+    for kind in (pkg.F32, pkg.F16):
+        a, b = (m.session(device_positions=320, kv_type=kind, weights=w) for w in (False, True))
+        assert np.array_equal(a.forward(tokens), b.forward(tokens))
+        assert np.array_equal(a.generate_greedy([7], 12)[0], b.generate_greedy([7], 12)[0])
+
+
+@pytest.mark.parametrize("variable", ["LLAMA_HIP_DECODE_EAGER", "LLAMA_HIP_DECODE_UNFUSED", "LLAMA_HIP_DECODE_STEP_PREFILL"])
+def test_the_sessions_other_ways(pkg, llama, model, monkeypatch, variable):
+    m, _ = model
+    prompt = np.random.default_rng(24).integers(0, 512, 50).tolist()
+    want, _, _ = m.session(device_positions=80, kv_type=pkg.F32, window=20, sinks=4).generate_greedy(prompt, 16)
+    monkeypatch.setenv(variable, "1")
+    got, _, _ = m.session(device_positions=80, kv_type=pkg.F32, window=20, sinks=4).generate_greedy(prompt, 16)
+    assert got.tolist() == want.tolist()
+
+
+def test_eviction_refusals(pkg, llama, model):
+    m, _ = model
+    for s in (m.session(), m.session(device_positions=16), m.session(device_positions=16, kv_type=pkg.F16)):
+        with pytest.raises(llama.LlamaError, match="keeps weights"):
+            s.evict(4)
+    s = m.session(device_positions=32, kv_type=pkg.F16, weights=True)
+    s.forward(list(range(20)))
+    with pytest.raises(llama.LlamaError, match="exceed those to keep"):
+        s.evict(10, 6, 6)
+    assert s.evict(10, 5, 5) == 10

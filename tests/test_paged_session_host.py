@@ -60,3 +60,18 @@ def test_head_sizes(pkg, llama, tmp_path):
     path = tmp_path / "narrow.gguf"
     llama.write_synthetic_llama(path, n_layer=1, n_embd=768, n_head=64, n_head_kv=64, n_ff=256, n_vocab=256, block_type=8, embd_type=8, output_type=8)
     both(llama.Llama(path=path, products=llama.CALLBACK, matmul=lambda *a: None), "multiple of 8", llama, kv_type=pkg.F32)
+
+
+def test_a_bounded_cache(pkg, llama, model):
+    for kw, match in ((dict(window=4, weights=True), "without a window"), (dict(cache_positions=17), "more positions than the session"),
+                      (dict(cache_positions=HUGE), "more positions than the session"), (dict(cache_positions=16, weights=True), "resident product route")):
+        with pytest.raises(llama.LlamaError, match=match):
+            model.session(device_positions=16, kv_type=pkg.F16, **kw)
+    for kw in (dict(weights=True), dict(cache_positions=8)):
+        with pytest.raises(llama.LlamaError, match="kv_type"):
+            model.session(device_positions=16, **kw)
+    # positions beyond the cache cost no rows of it
+    with pytest.raises(llama.LlamaError, match="resident product route"):
+        model.session(device_positions=(1 << 29) + 16, kv_type=pkg.F16, cache_positions=1 << 20)
+    with pytest.raises(llama.LlamaError, match="keeps weights"):
+        model.session().evict(4)
