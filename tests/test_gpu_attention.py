@@ -678,3 +678,20 @@ def test_few_tokens_behind_a_long_history(gpu, f16, tokens):
     q = rng.normal(0, 1, (tokens, 4, 128)).astype(np.float32)
     want, tol, _ = c.attend(0, q, 128 ** -0.5, [0, tokens])
     check(attend(gpu, c, 0, q, np.float32(128 ** -0.5)), want, tol + 1e-7 * np.abs(want))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n", [20, 33, 64])
+def test_one_long_sequence_among_short_ones(gpu, f16, n):
+    """Units that nearly fill, just pass and far pass the compute units, one of them with most of the positions."""
+    rng = np.random.default_rng(n)
+    lens = [40 + i for i in range(n)]
+    lens[n // 2], lens[1] = 6000, 1
+    c = Paged(rng, f16, 1, 8, 16, 16, lens, weights=True).up()
+    q = rng.normal(0, 1, (n, 8, 16)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, 0.25)
+    check(attend(gpu, c, 0, q, 0.25, weights=True), want, tol)
+    w, w_tol = c.weigh(0, sums, 1.0)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert np.all(np.abs(after[held] - w[held]) <= w_tol[held])
