@@ -695,3 +695,25 @@ def test_one_long_sequence_among_short_ones(gpu, f16, n):
     after = c.down()[2]
     held = ~np.isnan(w)
     assert np.all(np.abs(after[held] - w[held]) <= w_tol[held])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_that_share_blocks(gpu, hip, f16, new):
+    """A common beginning in the same blocks: attention reads them for both, and an eviction into other blocks takes from them twice."""
+    rng = np.random.default_rng(41 + new)
+    c = Paged(rng, f16, 1, 2, 64, 16, [320, 200], weights=True, extra_blocks=2 * 8)
+    c.tables[1, :10] = c.tables[0, :10]  # 160 positions
+    starts = [0, new, 2 * new]
+    c.up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (2 * new, 4, 64)).astype(np.float32)
+    want, tol, _ = c.attend(0, q, 0.125, starts)
+    check(attend(gpu, c, 0, q, 0.125), want, tol)
+    dst = c.free[:16].reshape(2, 8).astype(np.uint32)
+    dd, out = hip.DeviceBuffer.from_numpy(dst), hip.DeviceBuffer(8)
+    gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 128, 4, 16, dd.ptr, 8, out.ptr)
+    hip.device_synchronize()
+    want_len, k, v, w = c.evict([0], 128, 4, 16, dst)
+    assert out.to_numpy(np.uint32).tolist() == want_len.tolist()
+    for got, want in zip(c.down(), (k, v, w)):
+        assert same_bits(got, want)
