@@ -717,3 +717,36 @@ def test_sequences_that_share_blocks(gpu, hip, f16, new):
     assert out.to_numpy(np.uint32).tolist() == want_len.tolist()
     for got, want in zip(c.down(), (k, v, w)):
         assert same_bits(got, want)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_a_captured_call_follows_its_row_starts(gpu, hip, f16):
+    """Many rows, with weights, replayed with other starts and lengths: rows of nobody stay as they are, the others equal the eager call."""
+    rng = np.random.default_rng(51)
+    c = Paged(rng, f16, 1, 2, 64, 16, [640, 500, 90], weights=True, garbage=0.0).up([0, 24, 48, 72], max_new=40, n_tokens=80, max_len=640)
+    q, stream = hip.DeviceBuffer.from_numpy(rng.normal(0, 1, (80, 8, 64)).astype(np.float32)), hip.Stream()
+    out = hip.DeviceBuffer(80 * 8 * 64 * 4)
+    hip.device_synchronize()
+
+    def enqueue(s):
+        gpu.attn_device(c.cache, c.seqs, 0, 8, q.ptr, out.ptr, 0.125, weights=True, decay=0.5, stream=s.ptr)
+
+    enqueue(stream)
+    stream.synchronize()
+    graph = hip.Graph(stream, enqueue)
+    for starts, lens in (([0, 24, 48, 72], [640, 500, 90]), ([3, 3, 43, 44], [640, 77, 90]), ([0, 40, 80, 80], [40, 499, 1]), ([10, 10, 10, 10], [1, 1, 1]), ([79, 80, 80, 80], [600, 0, 0])):
+        got = []
+        for run in (enqueue, lambda s: graph.launch(), enqueue, lambda s: graph.launch()):
+            c.ds.upload(np.array(starts, np.uint32)), c.dl.upload(np.array(lens, np.uint32)), c.dw.upload(c.w)
+            out.fill_byte(0x22)
+            hip.device_synchronize()
+            run(stream)
+            stream.synchronize()
+            got.append((out.to_numpy(np.uint32).reshape(80, -1), c.down()[2].view(np.uint32)))
+        for o, w in got[1:]:
+            assert np.array_equal(o, got[0][0]) and np.array_equal(w, got[0][1]), starts
+        mine = np.zeros(80, bool)
+        mine[starts[0]:starts[-1]] = True
+        assert np.all(got[0][0][~mine] == 0x22222222) and np.all(np.any(got[0][0][mine] != 0x22222222, axis=1))
+    graph.destroy()
+    stream.destroy()
