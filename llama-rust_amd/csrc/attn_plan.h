@@ -108,6 +108,18 @@ NH_ATTN_HD uint32_t kv_row(const KvPlace &k, const uint32_t *table, uint32_t hea
     return id * k.block_rows + head_rows + (t - e * k.kv_block.d);
 }
 
+// The many-row kernels keep a row of K or V in LDS as 16-byte pieces, attn_pitch of them; their registers take dp head elements.
+constexpr uint32_t attn_piece(bool half) { return half ? 8 : 4; }  // head elements of a piece
+constexpr uint32_t attn_many_dims(bool half, uint32_t d) {
+    return d <= 64 ? 64 : half && d <= 96 ? 96 : d <= 128 ? 128 : half && d <= 192 ? 192 : 256;
+}
+constexpr uint32_t attn_pitch(bool half, uint32_t dp) { return half ? (dp > 128 ? 32 : dp > 64 ? 16 : 8) : dp / 4; }
+// Whether piece c of a place in LDS is loaded: only what the row has, d elements.  Where dp == d is known but the place is wider than the
+// row (f16 heads of 96 and 192), the pieces behind it are the next row's or, behind the last row, nobody's.
+NH_ATTN_HD bool attn_brings(bool half, uint32_t dp, uint32_t d, uint32_t c) {
+    return (dp == d && attn_pitch(half, dp) * attn_piece(half) == dp) || c * attn_piece(half) < d;
+}
+
 // ------------------------------------------------------------------ checks: a code and a message, LNH_OK and null if fine
 struct AttnCheck {
     int code;

@@ -208,7 +208,22 @@ static void seen_by() {
                 }
 }
 
+// What the many-row kernels load of a row lies within it, and of what they multiply, everything else is cleared instead.
+static void pieces() {
+    for (const bool half : {false, true})
+        for (uint32_t d = 8; d <= nh::ATTN_MAX_HEAD_DIM; d += 8) {
+            const uint32_t dp = nh::attn_many_dims(half, d), piece = nh::attn_piece(half), pitch = nh::attn_pitch(half, dp);
+            CHECK(dp >= d && dp % 32 == 0 && pitch * piece >= dp);
+            for (uint32_t c = 0; c < pitch; c++) {
+                const bool there = (c + 1) * piece <= d;
+                CHECK(nh::attn_brings(half, dp, d, c) == there);
+                if (!there && c < dp / piece) CHECK(dp != d);  // the kernels clear the places where dp != d
+            }
+        }
+}
+
 int main() {
+    pieces();
     seen_by();
     division();
     tiles();
