@@ -750,3 +750,40 @@ def test_a_captured_call_follows_its_row_starts(gpu, hip, f16):
         assert np.all(got[0][0][~mine] == 0x22222222) and np.all(np.any(got[0][0][mine] != 0x22222222, axis=1))
     graph.destroy()
     stream.destroy()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("d,block", [(40, 16), (80, 7), (96, 16), (136, 16), (64, 16)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_weights_of_few_rows_beside_keys_of_minus_infinity(gpu, f16, d, block, new):
+    """A key whose first element is -infinity against positive queries scores -infinity: it counts nothing and gets weight 0, the
+    others what the softmax without it gives them - also where the head ends inside a lane's piece and the first one is read instead."""
+    rng = np.random.default_rng(d + new)
+    heads, n, out_of = 4, 50, (3, 20, 44)
+    c = Paged(rng, f16, 1, 1, d, block, [n, n], weights=True, garbage=0.0)
+    for t in out_of:
+        c.k[c.tables[0, t // block], 0, 0, t % block, 0] = -np.inf
+    c.up([0, new, 2 * new] if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (2 * new, heads, d)).astype(np.float32)
+    q[:, :, 0] = np.abs(q[:, :, 0]) + 0.5
+    got = attend(gpu, c, 0, q, np.float32(d ** -0.5), weights=True, decay=0.5)
+    after = c.down()[2]
+    for b in range(2):
+        k, v = (np.array([x[c.tables[b, t // block], 0, 0, t % block] for t in range(n)], np.float64) for x in (c.k, c.v))
+        want, tol = np.zeros(n), np.zeros(n)
+        for i in range(new):
+            seen = np.array([t for t in range(n - new + i + 1) if b == 1 or t not in out_of])
+            for h in range(heads):
+                qr = q[b * new + i, h].astype(np.float64)
+                s = k[seen] @ qr * float(np.float32(d ** -0.5))
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                # as Paged.attend and Paged.weigh have them
+                rel = (2 * (d + 24) * (np.abs(k[seen]) @ np.abs(qr)).max() * d ** -0.5 + len(seen) + 80) * 2.0 ** -23
+                assert np.all(np.abs(got[b * new + i, h] - p @ v[seen]) <= rel * (p @ np.abs(v[seen])) + 1e-37), (b, i, h)
+                want[seen] += p
+                tol[seen] += (rel + new * heads * 2.0 ** -23) * p + 2.0 ** -120
+        for t in range(n):
+            at = c.tables[b, t // block], 0, 0, t % block
+            total = 0.5 * float(c.w[at]) + want[t]
+            assert abs(after[at] - total) <= tol[t] + 2 * 2.0 ** -24 * total, (b, t, after[at], total)
