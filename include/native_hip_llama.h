@@ -93,8 +93,8 @@ int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32
 /* The cache of a paged session with weights cut to `keep` positions, if it holds more: the first `first` of them, the last `recent`
  * and of those between the ones of the largest weight, for every layer and K/V head (lnh_kv_evict_device).  Later tokens see
  * what stays; keys keep the rotation of their own position and positions go on counting, up to max_positions.  *cached
- * (may be NULL): positions the cache holds now.  lnm_prompt reuses such a session's cache for a prompt that goes on where it is, and starts
- * anew for any other. */
+ * (may be NULL): positions the cache holds now.  lnm_prompt reuses the cache of a session with weights for a prompt that goes on where it is,
+ * and starts anew for any other, evicted or not: weights are those that the sequence's own tokens gave. */
 int lnm_session_evict(lnm_session *session, size_t keep, size_t first, size_t recent, size_t *cached);
 /* A device session for `n_sequences` (at most 128) independent sequences of up to `max_positions` each, decoded
  * together: every step processes one token of every sequence, the weight products as one multi-token product

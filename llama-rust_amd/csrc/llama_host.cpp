@@ -1442,7 +1442,8 @@ int lnm_prompt(lnm_session *session, const uint32_t *tokens, size_t n, float *lo
     if (session->ids.size() == session->past)  // ids that do not cover the cache are no basis for reuse
         while (lcp < session->ids.size() && lcp < n && session->ids[lcp] == tokens[lcp]) lcp++;
     if (prefix_hit) *prefix_hit = lcp;
-    if (session->dev && device_dropped(session) != 0 && (lcp < session->past || lcp == n)) {  // what an eviction left is no prefix: from the start
+    // what an eviction left is no prefix, and weights that tokens gave cannot be taken back, of the last one either: from the start
+    if (session->dev && device_keeps_weights(session) && (lcp < session->past || lcp == n)) {
         if (device_restart(session) != 0) return 1;
         lcp = 0;
         if (prefix_hit) *prefix_hit = 0;

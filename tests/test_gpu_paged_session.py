@@ -329,3 +329,35 @@ def test_eviction_refusals(pkg, llama, model):
     with pytest.raises(llama.LlamaError, match="exceed those to keep"):
         s.evict(10, 6, 6)
     assert s.evict(10, 5, 5) == 10
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_weights_are_those_of_the_tokens_that_are_there(pkg, llama, model, half):
+    """A prompt that leaves another one's path, or repeats it, before any eviction: what an eviction then keeps is what it keeps in a session
+    that saw the second prompt alone - tokens that are no longer there, or were run again, count nothing."""
+    m, _ = model
+    kind = pkg.F16 if half else pkg.F32
+    first = np.random.default_rng(25).integers(0, 512, 90).tolist()
+    tail = np.random.default_rng(26).integers(0, 512, 6).tolist()
+
+    def session():
+        return m.session(device_positions=160, kv_type=kind, weights=True)
+
+    for second in (first[:50] + [7, 8, 9, 10], first, first[:70], first[:1]):
+        s, alone = session(), session()
+        s.prompt(first)
+        for t in tail[:3]:
+            s.forward([t])
+        got, hit = s.prompt(second)
+        want, _ = alone.prompt(second)
+        assert hit == 0 and np.array_equal(got, want)
+        keep = len(second) // 2
+        assert s.evict(keep, 0, 1 if keep else 0) == alone.evict(keep, 0, 1 if keep else 0) == keep
+        for t in tail:
+            assert np.array_equal(s.forward([t]), alone.forward([t]))
+    # one that goes on where the cache is keeps it, evicted or not
+    s = session()
+    s.prompt(first)
+    assert s.prompt(first + tail)[1] == len(first)
+    s.evict(40, 4, 4)
+    assert s.prompt(first + tail + [3])[1] == len(first + tail)
