@@ -787,3 +787,22 @@ def test_weights_of_few_rows_beside_keys_of_minus_infinity(gpu, f16, d, block, n
             at = c.tables[b, t // block], 0, 0, t % block
             total = 0.5 * float(c.w[at]) + want[t]
             assert abs(after[at] - total) <= tol[t] + 2 * 2.0 ** -24 * total, (b, t, after[at], total)
+
+
+@pytest.mark.parametrize("heads,d,new,lens", [(4, 64, 1, [200, 4, 3000]), (2, 40, 1, [77, 1]), (4, 128, 20, [300, 25]), (8, 64, 40, [1200, 41]), (2, 200, 30, [100, 30])])
+def test_values_whose_sum_passes_f32(gpu, heads, d, new, lens):
+    """Values near the largest f32: their weighted sum before it is divided is beyond it, their mean is not."""
+    rng = np.random.default_rng(d + new)
+    starts = [new * i for i in range(len(lens) + 1)]
+    c = Paged(rng, False, 1, 1, d, 16, lens, weights=True)
+    held = ~np.isnan(c.v)
+    c.v[held] = (np.clip(c.v[held].astype(np.float64) * 4e37 + 2e38, -3.2e38, 3.2e38)).astype(np.float32)
+    c.up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (starts[-1], heads, d)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, d ** -0.5, starts)
+    got = attend(gpu, c, 0, q, np.float32(d ** -0.5), weights=True, decay=1.0)
+    check(got, want, tol + 1e-7 * np.abs(want))
+    w, w_tol = c.weigh(0, sums, 1.0)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert np.all(np.abs(after[held] - w[held]) <= w_tol[held] + 2e-7 * w[held])
