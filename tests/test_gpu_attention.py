@@ -806,3 +806,42 @@ def test_values_whose_sum_passes_f32(gpu, heads, d, new, lens):
     after = c.down()[2]
     held = ~np.isnan(w)
     assert np.all(np.abs(after[held] - w[held]) <= w_tol[held] + 2e-7 * w[held])
+
+
+@pytest.mark.parametrize("d", [64, 40, 200])
+@pytest.mark.parametrize("new,lens", [(1, [300, 9, 2000]), (30, [400, 30, 77])])
+def test_products_beyond_f32_whose_scores_are_not(gpu, d, new, lens):
+    """q k over an f32 cache passes the largest f32 for about every other position, scale q k is a few units: no score is lost to an
+    infinity of either sign before the scale comes to it."""
+    rng = np.random.default_rng(d + new)
+    starts = [new * i for i in range(len(lens) + 1)]
+    c = Paged(rng, False, 1, 1, d, 16, lens, weights=True)
+    c.k *= np.float32(6e17)
+    c.up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (starts[-1], 4, d)).astype(np.float32) * np.float32(1e20)
+    scale = np.float32(1.2e-38)
+    assert np.mean(np.abs(q[:, 0].astype(np.float64) @ c.k[c.at(0, 0)][0, 0].astype(np.float64)) > 3.4e38) > 0.2
+    want, tol, sums = c.attend(0, q, float(scale), starts)
+    check(attend(gpu, c, 0, q, scale, weights=True, decay=0.5), want, tol)
+    w, w_tol = c.weigh(0, sums, 0.5)
+    after = c.down()[2]
+    held = ~np.isnan(w)
+    assert np.all(np.abs(after[held] - w[held]) <= w_tol[held])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_one_position_has_all_the_weight_whatever_its_score(gpu, f16, new):
+    """A softmax over one position is 1 where its score is a finite f32, however far it lies below zero and however the factors of the
+    score are distributed."""
+    q0, k0, scale = (2.0 ** 125, -2.0 ** -24, 2.0 ** 17) if f16 else (1e20, -1e20, 1.2e-38)
+    rng = np.random.default_rng(new)
+    c = Paged(rng, f16, 1, 1, 64, 16, [new], weights=True)
+    for t in range(new):
+        c.k[c.at(0, t)] = k0
+    c.up([0, new] if new > 1 else None, max_new=new)
+    q = np.full((new, 4, 64), q0, np.float32)
+    out = attend(gpu, c, 0, q, np.float32(scale), window=1)
+    for t in range(new):
+        v = c.v[c.tables[0, t // 16], 0, 0, t % 16].astype(np.float64)
+        assert np.all(np.abs(out[t] - v) <= 2.0 ** -20 * np.abs(v)), t
