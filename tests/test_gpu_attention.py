@@ -845,3 +845,32 @@ def test_one_position_has_all_the_weight_whatever_its_score(gpu, f16, new):
     for t in range(new):
         v = c.v[c.tables[0, t // 16], 0, 0, t % 16].astype(np.float64)
         assert np.all(np.abs(out[t] - v) <= 2.0 ** -20 * np.abs(v)), t
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("size", [1e6, 3e8, 1e12, 1e30])
+@pytest.mark.parametrize("new,lens", [(1, [300, 1]), (8, [90, 2000]), (40, [64, 300, 40])])
+def test_rows_of_scores_far_from_zero(gpu, f16, size, new, lens):
+    """Scores that f32 holds in steps of more than one: where the largest leads by many steps the row is that position's value, anywhere it is
+    one between the values."""
+    rng = np.random.default_rng(new)
+    starts = [new * i for i in range(len(lens) + 1)]
+    c = Paged(rng, f16, 1, 1, 64, 16, lens).up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (starts[-1], 4, 64)).astype(np.float32) * np.float32(size)
+    got = attend(gpu, c, 0, q, 0.125).astype(np.float64)
+    led = 0
+    for b, n in enumerate(lens):
+        k, v = (np.array([x[c.at(b, t)][0, 0] for t in range(n)], np.float64) for x in (c.k, c.v))
+        for i in range(new):
+            for h in range(4):
+                row, here = starts[b] + i, n - new + i + 1
+                assert np.all(np.isfinite(got[row, h])) and np.all(np.abs(got[row, h]) <= np.abs(v[:here]).max(axis=0) * (1 + 2.0 ** -20)), (b, i, h)
+                s = k[:here] @ q[row, h].astype(np.float64) * 0.125
+                first = int(np.argmax(s))
+                # an f32 score of 64 products, q in 22 bits, is off by less than 100 parts in 2^22 of their sizes' sum; 30 units more leave
+                # nothing to the others
+                off = 100 * 2.0 ** -22 * (np.abs(k[:here]) @ np.abs(q[row, h].astype(np.float64))).max() * 0.125
+                if here == 1 or np.sort(s)[-2] < s[first] - 2 * off - 30:
+                    led += 1
+                    assert np.all(np.abs(got[row, h] - v[first]) <= 2.0 ** -20 * np.abs(v[first]).max()), (b, i, h)
+    assert led >= starts[-1] * 4 // 3
