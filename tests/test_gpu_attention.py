@@ -874,3 +874,28 @@ def test_rows_of_scores_far_from_zero(gpu, f16, size, new, lens):
                     led += 1
                     assert np.all(np.abs(got[row, h] - v[first]) <= 2.0 ** -20 * np.abs(v[first]).max()), (b, i, h)
     assert led >= starts[-1] * 4 // 3
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e5, 1e12, 1e30])
+@pytest.mark.parametrize("heads,new,lens", [(4, 1, [300, 1]), (4, 8, [90, 500]), (4, 40, [64, 300, 40]), (2, 300, [310])])
+def test_a_row_s_weights_sum_to_one(gpu, f16, size, heads, new, lens):
+    """Whatever the scores' size, what a row gives is one in all: the weights are formed by the numbers that its softmax was.  Equal
+    positions share alike."""
+    rng = np.random.default_rng(new)
+    starts = [new * i for i in range(len(lens) + 1)]
+    c = Paged(rng, f16, 1, 1, 64, 16, lens, weights=True)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            c.k[c.at(b, t)] = c.k[c.at(b, t % 7)]
+    c.up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (starts[-1], heads, 64)).astype(np.float32) * np.float32(size)
+    attend(gpu, c, 0, q, 0.125, weights=True, decay=0.0)
+    after = c.down()[2].astype(np.float64)
+    for b, n in enumerate(lens):
+        w = np.array([after[c.at(b, t)][0, 0] for t in range(n)])
+        # an exponent of a probability that counts is below 32, rounded to 2^-20 at the most, twice; sums of n numbers and their quotient
+        rel = 2 * np.log(2) * 2.0 ** -20 + (n + 80) * 2.0 ** -23
+        assert abs(w.sum() - new * heads) <= rel * new * heads, (b, w.sum())
+        for t in range(7, n - new):  # seen by every token, like the equal one before
+            assert abs(w[t] - w[t % 7]) <= 2 * rel * w[t % 7] + 2.0 ** -100, (b, t)
