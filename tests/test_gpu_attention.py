@@ -899,3 +899,24 @@ def test_a_row_s_weights_sum_to_one(gpu, f16, size, heads, new, lens):
         assert abs(w.sum() - new * heads) <= rel * new * heads, (b, w.sum())
         for t in range(7, n - new):  # seen by every token, like the equal one before
             assert abs(w[t] - w[t % 7]) <= 2 * rel * w[t % 7] + 2.0 ** -100, (b, t)
+
+
+def test_an_error_of_the_caller_s_is_not_the_call_s(gpu, hip):
+    """A failed HIP call of the program before, which it has not looked at, does not make the operators fail."""
+    rng = np.random.default_rng(3)
+    c = Paged(rng, False, 1, 1, 64, 16, [50, 20], weights=True, garbage=0.0).up()
+    q = rng.normal(0, 1, (2, 2, 64)).astype(np.float32)
+    want, tol, _ = c.attend(0, q, 0.125)
+    dq, out, new = hip.DeviceBuffer.from_numpy(q), hip.DeviceBuffer(q.nbytes), hip.DeviceBuffer(8)
+    kv = hip.DeviceBuffer.from_numpy(np.ones(128, np.float32))
+    for fails in (lambda: hip.rt().hipSetDevice(1000), lambda: hip.rt().hipMemcpy(None, None, 16, hip.H2D)):
+        for call in (lambda: gpu.attn_device(c.cache, c.seqs, 0, 2, dq.ptr, out.ptr, 0.125, weights=True),
+                     lambda: gpu.kv_evict_device(c.cache, c.seqs, 0, 1, 60, 0, 0, 0, 0, new.ptr),
+                     lambda: gpu.kv_store_device(c.cache, c.seqs, 0, kv.ptr, kv.ptr)):
+            c.dk.upload(c.k), c.dv.upload(c.v)
+            hip.device_synchronize()
+            assert fails() != 0
+            call()
+            hip.device_synchronize()
+    check(out.to_numpy(np.float32).reshape(q.shape), want, tol)
+    assert new.to_numpy(np.uint32).tolist() == [50, 20]
