@@ -1,4 +1,5 @@
-// Host-callable launchers of the paged-cache operators (attn.hip).  Arguments have passed attn_plan.h's checks.
+// Host-callable launchers of the paged-cache operators (attn.hip).  Arguments have passed attn_plan.h's checks, and a call is launched only
+// if .._fits() says that its launches hold it, which also says what workspace the launch takes.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -13,6 +14,7 @@ struct KvStoreCall {
     const float *k, *v;
     size_t k_stride, v_stride;
 };
+bool kv_store_fits(const KvStoreCall &c);
 hipError_t launch_kv_store(hipStream_t stream, const KvStoreCall &c);
 
 struct AttnCall {
@@ -27,8 +29,8 @@ struct AttnCall {
     bool weights;
     float decay;
 };
-// cus: compute units of the GPU.  ws holds at least attn_workspace_bytes() of the same call, 16-byte aligned.
-size_t attn_workspace_bytes(const AttnCall &c, uint32_t cus);
+// cus: compute units of the GPU.  ws holds at least *workspace bytes of the same call, 16-byte aligned.
+bool attn_fits(const AttnCall &c, uint32_t cus, size_t *workspace);
 hipError_t launch_attn(hipStream_t stream, const AttnCall &c, uint32_t cus, void *ws);
 
 struct KvEvictCall {
@@ -39,7 +41,7 @@ struct KvEvictCall {
     size_t dst_stride;
     uint32_t *new_lens;
 };
-size_t kv_evict_workspace_bytes(const KvEvictCall &c);
+bool kv_evict_fits(const KvEvictCall &c, size_t *workspace);
 hipError_t launch_kv_evict(hipStream_t stream, const KvEvictCall &c, uint32_t cus, void *ws);
 
 }  // namespace nh
