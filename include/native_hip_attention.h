@@ -72,7 +72,9 @@ int lnh_kv_store_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_
  * The caller sets the weight of a new position to zero before it is first counted (or passes decay 0).  Sequences
  * that share a block then race on its weights.
  * Uses the executor's workspace like lnh_gemm_device: calls of one executor on one stream at a time, and one call of
- * the largest shape before capturing. */
+ * the largest shape before capturing.  Weights take workspace by max_len, for scores or sums of each of its positions: up to 16 rows (new tokens
+ * times query heads of a key-value head) n_head * max_new * max_len floats a sequence, above that a float a position, key-value head and
+ * block of 64 to 256 rows.  Sequences go in parts where theirs together pass 1 GiB. */
 int lnh_attn_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, size_t n_head,
                     const float *device_q, size_t q_stride, float *device_out, size_t out_stride, float scale,
                     size_t window, size_t sinks, int weights, float decay, void *stream);

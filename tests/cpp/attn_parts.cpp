@@ -222,7 +222,23 @@ static void pieces() {
         }
 }
 
+// Sequences go in parts of nearly one size: few enough for few rows, with no more workspace for weights than there is to be, one at least.
+static void parts() {
+    for (const size_t n : {0, 1, 2, 64, 255, 256, 257, 300, 512, 513, 1000, 8192, 0x3fffff})
+        for (const bool few : {false, true})
+            for (const size_t bytes : {(size_t)0, (size_t)1, (size_t)1 << 20, ((size_t)1 << 24) + 1, (size_t)1 << 30, ((size_t)1 << 30) + 1, (size_t)1 << 50}) {
+                const size_t at_once = nh::attn_seqs_at_once(n, few, bytes);
+                CHECK(at_once <= n && (at_once >= 1 || n == 0));
+                if (few) CHECK(at_once <= 256);
+                if (at_once > 1) CHECK(at_once * bytes <= (size_t)1 << 30);
+                if (!few && n * bytes <= (size_t)1 << 30) CHECK(at_once == n);
+                if (few && n <= 256 && n * bytes <= (size_t)1 << 30) CHECK(at_once == n);
+                if (at_once) CHECK(n - (n - 1) / at_once * at_once + (n + at_once - 1) / at_once > at_once);  // the last part is short by less than there are parts
+            }
+}
+
 int main() {
+    parts();
     pieces();
     seen_by();
     division();

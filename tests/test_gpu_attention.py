@@ -920,3 +920,42 @@ def test_an_error_of_the_caller_s_is_not_the_call_s(gpu, hip):
             hip.device_synchronize()
     check(out.to_numpy(np.float32).reshape(q.shape), want, tol)
     assert new.to_numpy(np.uint32).tolist() == [50, 20]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 3])
+def test_sequences_in_several_parts(gpu, hip, f16, new):
+    """More sequences than a launch of few rows looks at, with rows of nobody before, behind and, by their starts, between; weights; captured and
+    replayed with other lengths."""
+    rng = np.random.default_rng(60 + new)
+    n, heads = 601, 4
+    lens = [int(rng.integers(new, 40)) if i % 50 else 700 for i in range(n)]
+    lens[7] = lens[300] = lens[600] = 0
+    starts = [5 + new * i for i in range(n + 1)] if new > 1 else None
+    c = Paged(rng, f16, 1, 2, 16, 16, lens, weights=True, garbage=0.0).up(starts, max_new=new, n_tokens=n * new + 9 if starts else n)
+    rows = n * new + 9 if starts else n
+    q = rng.normal(0, 1, (rows, heads, 16)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, 0.25, starts)
+    got = attend(gpu, c, 0, q, 0.25, weights=True, decay=0.5)
+    mine = slice(5, 5 + n * new) if starts else slice(0, n)
+    check(got[mine], want[mine], tol[mine])
+    if starts:
+        assert np.all(got[:5] == 7.25) and np.all(got[5 + n * new:] == 7.25)
+    w, w_tol = c.weigh(0, sums, 0.5)
+    after = c.down()[2]
+    assert np.all(np.abs(after - w) <= w_tol)
+    dq, out, stream = hip.DeviceBuffer.from_numpy(q), hip.DeviceBuffer(q.nbytes), hip.Stream()
+    hip.device_synchronize()
+    graph = hip.Graph(stream, lambda s: gpu.attn_device(c.cache, c.seqs, 0, heads, dq.ptr, out.ptr, 0.25, weights=True, decay=0.0, stream=s.ptr))
+    for change in (lens, [min(x, 3 + i % 30) for i, x in enumerate(lens)], lens):
+        c.lens = np.array(change, np.uint32)
+        c.dl.upload(c.lens)
+        hip.device_synchronize()
+        eager = attend(gpu, c, 0, q, 0.25, weights=True, decay=0.0)
+        eager_w = c.down()[2]
+        out.fill_byte(0)
+        graph.launch()
+        stream.synchronize()
+        assert np.array_equal(out.to_numpy(np.float32).reshape(q.shape)[mine], eager[mine]) and np.array_equal(c.down()[2], eager_w)
+    graph.destroy()
+    stream.destroy()
