@@ -86,7 +86,9 @@ int lnh_attn_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs
  * alike, and device_new_lens[b] (may be device_lens itself) becomes min(length, keep).  device_dst_tables NULL or
  * device_tables itself: in place.  Otherwise sequences that need no cut are copied as they are, and the destination's
  * blocks must be none that any of the call's sequences reads.  In place, sequences must not share blocks.  Rows behind
- * the new lengths are left as they are.  device_starts is not looked at.  Uses the executor's workspace. */
+ * the new lengths are left as they are, and so is the new place of a position that stays though its block is not there: it is one of the
+ * sequence's positions from then on.  device_starts is not looked at.  Uses the executor's workspace: a word a layer, key-value head and
+ * position that may stay, sequences in parts as above. */
 int lnh_kv_evict_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t first_layer,
                         size_t n_layers, size_t keep, size_t first, size_t recent, const uint32_t *device_dst_tables,
                         size_t dst_stride, uint32_t *device_new_lens, void *stream);

@@ -959,3 +959,35 @@ def test_sequences_in_several_parts(gpu, hip, f16, new):
         assert np.array_equal(out.to_numpy(np.float32).reshape(q.shape)[mine], eager[mine]) and np.array_equal(c.down()[2], eager_w)
     graph.destroy()
     stream.destroy()
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_sequences_in_parts_by_their_workspace(pkg, hip, new):
+    """Bounds far beyond the lengths: weights and what an eviction looks up would take more than a GiB for all sequences together."""
+    rng = np.random.default_rng(70 + new)
+    n, far = 300, 65536  # table entries of 16 positions
+    lens = [int(rng.integers(new, 60)) for i in range(n)]
+    starts = [new * i for i in range(n + 1)]
+    c = Paged(rng, True, 1, 1, 8, 16, lens, weights=True, garbage=0.0, extra_blocks=4 * n)
+    tables = np.full((n, far), NOWHERE, np.uint32)
+    tables[:, :c.stride] = c.tables
+    c.tables, c.stride = tables, far
+    c.up(starts if new > 1 else None, max_new=new, max_len=far * 16)
+    g = pkg.HipGemv(0)
+    q = rng.normal(0, 1, (n * new, 2, 8)).astype(np.float32)
+    want, tol, sums = c.attend(0, q, 0.25, starts)
+    check(attend(g, c, 0, q, 0.25, weights=True, decay=1.0), want, tol)
+    w, w_tol = c.weigh(0, sums, 1.0)
+    after = c.down()[2]
+    assert np.all(np.abs(after - w) <= w_tol)
+    c.w = after
+    dst = np.full((n, far), NOWHERE, np.uint32)
+    dst[:, :4] = c.free[:4 * n].reshape(n, 4)
+    dd, out = hip.DeviceBuffer.from_numpy(dst), hip.DeviceBuffer(4 * n)
+    g.kv_evict_device(c.cache, c.seqs, 0, 1, far * 16, 0, 0, dd.ptr, far, out.ptr)
+    hip.device_synchronize()
+    want_len, k, v, w = c.evict([0], far * 16, 0, 0, dst)
+    assert out.to_numpy(np.uint32).tolist() == want_len.tolist()
+    for got, expect in zip(c.down(), (k, v, w)):
+        assert same_bits(got, expect)
+    g.close()
