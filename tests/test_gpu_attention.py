@@ -991,3 +991,77 @@ def test_sequences_in_parts_by_their_workspace(pkg, hip, new):
     for got, expect in zip(c.down(), (k, v, w)):
         assert same_bits(got, expect)
     g.close()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("most,news,lens", [(2, [5, 1, 2], [9, 4, 30]), (3, [5, 9, 0], [200, 9, 40]), (40, [45, 70, 3], [45, 300, 60])])
+def test_new_tokens_beyond_their_bound_are_left_out(gpu, hip, f16, most, news, lens):
+    """A sequence with more new tokens than max_new: the first max_new of them are stored and attend from where they stand, the others' rows,
+    places and weights stay as they are; so do tokens behind n_tokens."""
+    rng = np.random.default_rng(most)
+    starts = np.concatenate([[0], np.cumsum(news)]).astype(int)
+    rows = int(starts[-1])
+    c = Paged(rng, f16, 1, 2, 64, 16, lens, weights=True, garbage=0.0).up(starts, max_new=most)
+    dt = c.k.dtype
+    k, v = (rng.normal(0, 1, (rows, 2, 64)).astype(np.float32) for _ in range(2))
+    dk, dv = hip.DeviceBuffer.from_numpy(k), hip.DeviceBuffer.from_numpy(v)
+    gpu.kv_store_device(c.cache, c.seqs, 0, dk.ptr, dv.ptr)
+    taken = np.zeros(rows, bool)
+    for b, n in enumerate(news):
+        for i in range(min(n, most)):
+            taken[starts[b] + i] = True
+            at = c.at(b, lens[b] - n + i)
+            c.k[at[0], 0, :, at[3]], c.v[at[0], 0, :, at[3]] = k[starts[b] + i].astype(dt), v[starts[b] + i].astype(dt)
+    q = rng.normal(0, 1, (rows, 8, 64)).astype(np.float32)
+    got = attend(gpu, c, 0, q, 0.125, weights=True, decay=0.5)
+    got_k, got_v, after = c.down()
+    assert same_bits(got_k, c.k) and same_bits(got_v, c.v)
+    want, tol, _ = c.attend(0, q, 0.125, starts)
+    check(got[taken], want[taken], tol[taken])
+    assert np.all(got[~taken] == 7.25)
+    # the taken rows' weights: of the sequences without the others' rows, at the positions that they stand at
+    total = 0.5 * c.w.astype(np.float64)
+    for b, n in enumerate(news):
+        if n == 0:
+            continue
+        cut = Paged.__new__(Paged)
+        cut.__dict__.update(c.__dict__)
+        cut.lens = np.array([lens[b] - n + min(n, most)], np.uint32)
+        cut.tables = c.tables[b:b + 1]
+        _, _, sums = cut.attend(0, q[starts[b]:starts[b] + min(n, most)], 0.125, [0, min(n, most)])
+        for (_, h), (pos, ws, wt) in sums.items():
+            for t, x, y in zip(pos, ws, wt):
+                i = c.tables[b, t // 16], 0, h, t % 16
+                total[i] += x
+                assert abs(after[i] - total[i]) <= y + 2 * 2.0 ** -24 * total[i], (b, h, t)
+        for t in range(lens[b] - n + min(n, most), lens[b]):  # positions of tokens that were left out: seen by none
+            i = c.tables[b, t // 16], 0, slice(None), t % 16
+            assert np.all(after[i] == (0.5 * c.w[i]).astype(np.float32))
+    # n_tokens cuts the last sequence's rows, which then are the positions' last ones
+    less = rows - 1
+    c.seqs.n_tokens = less
+    short = [int(min(s, less)) for s in starts]
+    want, tol, _ = c.attend(0, q[:less], 0.125, short)
+    got = attend(gpu, c, 0, q, 0.125)
+    mine = np.zeros(rows, bool)
+    for b in range(len(news)):
+        mine[short[b]:short[b] + min(short[b + 1] - short[b], most)] = True
+    check(got[mine], want[mine[:less]], tol[mine[:less]])
+    assert np.all(got[~mine] == 7.25)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_a_padded_batch(gpu, f16):
+    """Sequences that are only there to fill a fixed size: no positions, no rows, tables that name nothing."""
+    rng = np.random.default_rng(81)
+    for new, starts in ((1, None), (30, [0, 30, 30, 60, 60, 60])):
+        lens = [50, 0, 75, 0, 0]
+        c = Paged(rng, f16, 1, 2, 64, 16, lens, weights=True, garbage=0.0)
+        c.tables[[1, 3, 4]] = NOWHERE
+        c.up(starts, max_new=new)
+        q = rng.normal(0, 1, (5 if starts is None else 60, 4, 64)).astype(np.float32)
+        want, tol, sums = c.attend(0, q, 0.125, starts)
+        got = attend(gpu, c, 0, q, 0.125, weights=True)
+        check(got, want, tol)
+        w, w_tol = c.weigh(0, sums, 1.0)
+        assert np.all(np.abs(c.down()[2] - w) <= w_tol)
