@@ -65,7 +65,8 @@ int lnh_kv_store_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_
  * floats.  A token that sees nothing gets zeros; so does one whose every score is -infinity.  What lies in positions
  * that a token does not see, infinities and NaN among it, does not reach its row.
  * Scores, the softmax and the sums are f32; over an f16 cache q and the probabilities enter the matrix cores as two
- * f16 parts each (22 bits).
+ * f16 parts each (22 bits).  A row that comes out not finite so, or of scores beyond 2^21 / log2(e), is computed again
+ * from the definition, its scores summed in 64 bits, at about a hundred times the time.
  * weights != 0 (needs device_w): for every position t below the length of a sequence with new tokens, per key-value head,
  * device_w = decay * device_w + the sum over the sequence's new tokens and the head's query heads of the softmax
  * probability they give t.  decay 1 sums over all calls, 0 keeps this call's alone, whatever the memory held before.

@@ -263,7 +263,7 @@ class Session:
     def prompt(self, tokens):
         """(logits of the last of `tokens`, reused prefix length): `tokens` as the whole sequence, keeping the
         cached positions of the longest prefix it shares with what the session has forwarded so far
-        (langtax/src/decode.rs:3956-3962)."""
+        (langtax/src/decode.rs:3956-3962); a session with weights keeps them only for a prompt that goes on where it is."""
         t = np.ascontiguousarray(tokens, dtype=np.uint32)
         logits = np.empty(self.model.hparams.n_vocab, dtype=np.float32)
         hit = C.c_size_t()
