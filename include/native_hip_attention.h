@@ -1,10 +1,10 @@
-/* native-hip: operators over a paged key-value cache in device memory - storing the rows of new tokens, attention
- * that reads the cache, eviction by accumulated attention weight.
+/* native-hip: operators over a paged key-value cache in device memory - storing the rows of new tokens, with the rotation by
+ * their positions on the way if wanted, attention that reads the cache, eviction by accumulated attention weight.
  *
  * The products of native_hip.h leave q, k and v of a step in HBM; these calls are what stands between them and the
  * output projection for a caller that keeps its own cache: the reference's attention over paged K/V
  * (langtax/src/decode.rs:11126-11197, 12059-12100; langtax/src/kv_page.rs:47-53, 410-438) runs on the host and has
- * neither an f16 cache, nor the window with first tokens, nor the eviction.
+ * neither an f16 or a 4-bit cache, nor the window with first tokens, nor the eviction.
  *
  * Conventions are those of native_hip.h: plain pointers and sizes, LNH_OK or an lnh_status, lnh_last_error(exec),
  * validation before anything is launched, no host synchronisation, `stream` a hipStream_t of the executor's GPU
@@ -26,8 +26,18 @@ extern "C" {
 #endif
 
 /* The cache: K and V as [n_blocks][n_layer][n_head_kv][kv_block][head_dim] of LNH_TYPE_F32 or LNH_TYPE_F16
- * (LNH_ERR_UNSUPPORTED otherwise), head_dim a multiple of 8, at most 256 (LNH_ERR_UNSUPPORTED otherwise), at most 2^31
- * rows of head_dim in all.  device_w, where weights are kept: [n_blocks][n_layer][n_head_kv][kv_block] f32, else NULL. */
+ * or, in 4 bits, LNH_TYPE_Q4_0 (LNH_ERR_UNSUPPORTED otherwise), head_dim a multiple of 8 (LNH_TYPE_Q4_0: of 32), at most 256
+ * (LNH_ERR_UNSUPPORTED otherwise), at most 2^31 rows of head_dim in all.  device_w, where weights are kept:
+ * [n_blocks][n_layer][n_head_kv][kv_block] f32, else NULL.
+ *
+ * LNH_TYPE_Q4_0: 32 elements of a row share an f16 scale d and have a code of 4 bits each; an element is (code - 8) d.  K and V
+ * are each [n_blocks][n_layer][n_head_kv][kv_block][head_dim / 2] bytes of codes - eight to a little-endian word, element 2 i of
+ * the eight at bit 4 i, element 2 i + 1 at bit 16 + 4 i - and behind them [n_blocks][n_layer][n_head_kv][head_dim / 32][kv_block]
+ * scales, 18 bytes for 32 elements in all.  Stored rows have d = -1/8 of the element of the largest size (the first of those),
+ * rounded to eight significant bits and to an f16, at most 8160, and the nearest codes, ties to even: every element is then an
+ * f16, and what the operators make of such a cache is what they make of an f16 cache of these values.  Larger numbers than 65280
+ * are held to it; 32 of which one is infinite or NaN are all NaN.  Scales that a caller writes itself should keep to eight bits:
+ * elements are rounded to f16. */
 typedef struct lnh_kv_cache {
     uint32_t ggml_type;
     uint32_t n_layer, n_head_kv, head_dim, kv_block, n_blocks;
@@ -58,13 +68,44 @@ typedef struct lnh_kv_seqs {
 int lnh_kv_store_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer,
                         const float *device_k, size_t k_stride, const float *device_v, size_t v_stride, void *stream);
 
+/* How queries and keys are turned by their position: pair i of a head's first n_rot elements (even, at most head_dim; 0: none is turned),
+ * (x, y) -> (x c - y s, x s + y c) with (c, s) the pair at device_angles + 2 * (position * angle_stride + i) (floats, 8-byte
+ * aligned; angle_stride in pairs).  Pairs are elements 2 i and 2 i + 1, or, with halves != 0, i and i + n_rot / 2.  A token's
+ * position is its place in its sequence or, where device_positions is not NULL, device_positions[row]; a position that is not
+ * below n_positions takes the last one's angles. */
+typedef struct lnh_rope {
+    const float *device_angles;
+    size_t angle_stride, n_positions;
+    uint32_t n_rot;
+    int halves;
+    const uint32_t *device_positions;
+} lnh_rope;
+
+/* The angles' cosines and sines of positions 0 .. n_positions - 1: pair i of n_rot / 2 turns by position * scale * base^(-2 i / n_rot),
+ * divided by device_divisors[i] where those are not NULL; formed in 64 bits, rounded to f32.  base and scale positive. */
+int lnh_rope_table_device(lnh_exec *exec, uint32_t n_rot, double base, double scale, const float *device_divisors, size_t n_positions,
+                          float *device_angles, size_t angle_stride, void *stream);
+
+/* lnh_kv_store_device with the rotation on the way: rows of device_q (n_head heads; n_head 0: none, device_q and device_q_out are not
+ * looked at) are turned into device_q_out (may be device_q itself, of the same stride), rows of device_k into K; V as it is.  rope
+ * NULL: nothing is turned.  Numbers are turned in 64 bits and rounded to f32, then to the cache's type.  Where the cache keeps
+ * weights, those of the new positions become zero.  A new token below position 0 keeps its row of device_q_out as it was. */
+int lnh_kv_append_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, const lnh_rope *rope, size_t n_head,
+                         const float *device_q, size_t q_stride, float *device_q_out, size_t q_out_stride, const float *device_k,
+                         size_t k_stride, const float *device_v, size_t v_stride, void *stream);
+
+/* What `layer` of the cache has for the new tokens, as f32 rows: lnh_kv_store_device's way back, for a prefix that goes to another cache or
+ * program.  A new token that stands nowhere (below position 0, or in a block that is not there) gets zeros. */
+int lnh_kv_load_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, float *device_k, size_t k_stride,
+                       float *device_v, size_t v_stride, void *stream);
+
 /* out = softmax(scale q K^T) V for every new token and each of n_head query heads (a multiple of n_head_kv; query
  * head h reads key-value head h * n_head_kv / n_head; 0 < scale <= 2^127), over `layer` of the cache: the new tokens' own rows have to be
  * stored before.  The token at position p sees position t where t <= p and, with window > 0, p - t < window or
  * t < sinks (sinks without a window: LNH_ERR_INVALID).  Rows of q and out are n_head * head_dim floats, strides in
  * floats.  A token that sees nothing gets zeros; so does one whose every score is -infinity.  What lies in positions
  * that a token does not see, infinities and NaN among it, does not reach its row.
- * Scores, the softmax and the sums are f32; over an f16 cache q and the probabilities enter the matrix cores as two
+ * Scores, the softmax and the sums are f32; over an f16 or a 4-bit cache q and the probabilities enter the matrix cores as two
  * f16 parts each (22 bits).  A row that comes out not finite so, or of scores beyond 2^21 / log2(e), is computed again
  * from the definition, its scores summed in 64 bits, at about a hundred times the time.
  * weights != 0 (needs device_w): for every position t below the length of a sequence with new tokens, per key-value head,

@@ -74,12 +74,28 @@ def build_selftest(verbose=False):
 
 class KvCache(C.Structure):
     """A paged K/V cache in the caller's device memory (lnh_kv_cache, include/native_hip_attention.h): k and v as
-    [n_blocks][n_layer][n_head_kv][kv_block][head_dim] of F32 or F16, w (0: none) the same without the last axis, f32."""
+    [n_blocks][n_layer][n_head_kv][kv_block][head_dim] of F32 or F16, or of Q4_0 as the header lays it out (codes, then scales; q4_0_bytes()
+    in all), w (0: none) the same without the last axis, f32."""
     _fields_ = [(n, C.c_uint32) for n in ("ggml_type", "n_layer", "n_head_kv", "head_dim", "kv_block", "n_blocks")] + \
                [(n, C.c_void_p) for n in ("device_k", "device_v", "device_w")]
 
     def __init__(self, ggml_type, n_layer, n_head_kv, head_dim, kv_block, n_blocks, k_ptr, v_ptr, w_ptr=0):
         super().__init__(ggml_type, n_layer, n_head_kv, head_dim, kv_block, n_blocks, k_ptr, v_ptr, w_ptr)
+
+
+def q4_0_bytes(n_layer, n_head_kv, head_dim, kv_block, n_blocks):
+    """Bytes of K, or of V, of a Q4_0 cache."""
+    return n_blocks * n_layer * n_head_kv * kv_block * head_dim // 32 * 18
+
+
+class Rope(C.Structure):
+    """The rotation of queries and keys (lnh_rope): angles as [n_positions][angle_stride] (cos, sin) pairs of f32 in device memory; pairs of elements
+    are adjacent or halves of the turned part apart; positions (0: a token's place) a u32 array, one a row."""
+    _fields_ = [("device_angles", C.c_void_p), ("angle_stride", C.c_size_t), ("n_positions", C.c_size_t), ("n_rot", C.c_uint32), ("halves", C.c_int),
+                ("device_positions", C.c_void_p)]
+
+    def __init__(self, angles_ptr, angle_stride, n_positions, n_rot, halves=False, positions_ptr=0):
+        super().__init__(angles_ptr, angle_stride, n_positions, n_rot, int(halves), positions_ptr)
 
 
 class KvSeqs(C.Structure):
@@ -185,9 +201,12 @@ def load_library():
                                       C.POINTER(u32), psz, psz]),
     }
     # include/native_hip_attention.h
-    pc, ps = C.POINTER(KvCache), C.POINTER(KvSeqs)
+    pc, ps, pr = C.POINTER(KvCache), C.POINTER(KvSeqs), C.POINTER(Rope)
     paged = {
         "lnh_kv_store_device": (C.c_int, [vp, pc, ps, sz, vp, sz, vp, sz, vp]),
+        "lnh_rope_table_device": (C.c_int, [vp, u32, C.c_double, C.c_double, vp, sz, vp, sz, vp]),
+        "lnh_kv_append_device": (C.c_int, [vp, pc, ps, sz, pr, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp]),
+        "lnh_kv_load_device": (C.c_int, [vp, pc, ps, sz, vp, sz, vp, sz, vp]),
         "lnh_attn_device": (C.c_int, [vp, pc, ps, sz, sz, vp, sz, vp, sz, C.c_float, sz, sz, C.c_int, C.c_float, vp]),
         "lnh_kv_evict_device": (C.c_int, [vp, pc, ps, sz, sz, sz, sz, sz, vp, sz, vp, vp]),
     }
@@ -465,6 +484,25 @@ class HipGemv:
         row = cache.n_head_kv * cache.head_dim
         self._check(self._lib.lnh_kv_store_device(self._h, C.byref(cache), C.byref(seqs), layer, k_ptr, row if k_stride is None else k_stride,
                                                   v_ptr, row if v_stride is None else v_stride, stream))
+
+    def rope_table_device(self, n_rot, base, n_positions, angles_ptr, angle_stride=None, scale=1.0, divisors_ptr=0, stream=0):
+        """Cosines and sines of every position's angles, for Rope; formed in 64 bits."""
+        self._check(self._lib.lnh_rope_table_device(self._h, n_rot, base, scale, divisors_ptr, n_positions, angles_ptr,
+                                                    n_rot // 2 if angle_stride is None else angle_stride, stream))
+
+    def kv_append_device(self, cache, seqs, layer, rope, n_head, q_ptr, q_out_ptr, k_ptr, v_ptr, q_stride=None, q_out_stride=None, k_stride=None,
+                         v_stride=None, stream=0):
+        """q of the new tokens turned by their positions into q_out (may be q), k turned and v into the cache; rope None: nothing is turned."""
+        row, kv = n_head * cache.head_dim, cache.n_head_kv * cache.head_dim
+        self._check(self._lib.lnh_kv_append_device(self._h, C.byref(cache), C.byref(seqs), layer, C.byref(rope) if rope is not None else None, n_head, q_ptr,
+                                                   row if q_stride is None else q_stride, q_out_ptr, row if q_out_stride is None else q_out_stride, k_ptr,
+                                                   kv if k_stride is None else k_stride, v_ptr, kv if v_stride is None else v_stride, stream))
+
+    def kv_load_device(self, cache, seqs, layer, k_ptr, v_ptr, k_stride=None, v_stride=None, stream=0):
+        """What the cache has for the new tokens, as f32 rows."""
+        row = cache.n_head_kv * cache.head_dim
+        self._check(self._lib.lnh_kv_load_device(self._h, C.byref(cache), C.byref(seqs), layer, k_ptr, row if k_stride is None else k_stride,
+                                                 v_ptr, row if v_stride is None else v_stride, stream))
 
     def attn_device(self, cache, seqs, layer, n_head, q_ptr, out_ptr, scale, q_stride=None, out_stride=None, window=0, sinks=0,
                     weights=False, decay=1.0, stream=0):

@@ -17,6 +17,25 @@ struct KvStoreCall {
 bool kv_store_fits(const KvStoreCall &c);
 hipError_t launch_kv_store(hipStream_t stream, const KvStoreCall &c);
 
+// The rotation on the way and q with it; launch_kv_load: k and v are written.
+struct KvAppendCall {
+    const lnh_kv_cache *cache;
+    const lnh_kv_seqs *seqs;
+    size_t layer;
+    const lnh_rope *rope;  // may be null
+    size_t n_head;
+    const float *q;
+    float *q_out;
+    size_t q_stride, q_out_stride;
+    const float *k, *v;
+    size_t k_stride, v_stride;
+};
+bool kv_append_fits(const KvAppendCall &c);
+hipError_t launch_kv_append(hipStream_t stream, const KvAppendCall &c);
+hipError_t launch_kv_load(hipStream_t stream, const KvAppendCall &c, float *k, float *v);
+hipError_t launch_rope_table(hipStream_t stream, uint32_t n_rot, double base, double scale, const float *divisors, size_t n_positions, float *angles,
+                             size_t stride);
+
 struct AttnCall {
     const lnh_kv_cache *cache;
     const lnh_kv_seqs *seqs;

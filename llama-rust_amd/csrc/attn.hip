@@ -24,10 +24,12 @@ using uint2v = uint32_t __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
+#include "attn_q4.inc"
 #include "attn_rows.inc"
 #include "attn_split.inc"
 #include "attn_chunk.inc"
 #include "attn_weights.inc"
+#include "kv_append.inc"
 #include "kv_store.inc"
 #include "kv_evict.inc"
 

@@ -141,11 +141,14 @@ inline bool attn_misaligned(const void *p, uintptr_t to) { return (reinterpret_c
 
 inline AttnCheck check_kv_cache(const lnh_kv_cache *c, bool weights) {
     if (!c) return {LNH_ERR_INVALID, "K/V cache description is null"};
-    if (c->ggml_type != LNH_TYPE_F32 && c->ggml_type != LNH_TYPE_F16) return {LNH_ERR_UNSUPPORTED, "the K/V cache is f32 or f16"};
+    if (c->ggml_type != LNH_TYPE_F32 && c->ggml_type != LNH_TYPE_F16 && c->ggml_type != LNH_TYPE_Q4_0)
+        return {LNH_ERR_UNSUPPORTED, "the K/V cache is f32 or f16 or q4_0"};
     if (c->n_layer == 0 || c->n_head_kv == 0 || c->head_dim == 0 || c->kv_block == 0 || c->n_blocks == 0)
         return {LNH_ERR_INVALID, "K/V cache dimensions must be positive"};
     if (c->head_dim % 8 != 0 || c->head_dim > ATTN_MAX_HEAD_DIM)
         return {LNH_ERR_UNSUPPORTED, "the K/V cache takes head sizes that are multiples of 8, at most 256"};
+    if (c->ggml_type == LNH_TYPE_Q4_0 && c->head_dim % 32 != 0)
+        return {LNH_ERR_UNSUPPORTED, "a q4_0 K/V cache takes head sizes that are multiples of 32"};
     size_t rows = 1;
     for (const uint32_t n : {c->n_layer, c->n_head_kv, c->kv_block, c->n_blocks}) {
         rows *= n;  // below 2^31 times at most 2^32
@@ -213,6 +216,43 @@ inline AttnCheck check_kv_store(const lnh_kv_cache *c, const lnh_kv_seqs *s, siz
     const size_t width = (size_t)c->n_head_kv * c->head_dim;
     r = check_rows(k, k_stride, width);
     return r.what ? r : check_rows(v, v_stride, width);
+}
+
+inline AttnCheck check_rope(const lnh_rope *r, size_t head_dim, size_t n_tokens) {
+    if (!r || r->n_rot == 0) return {LNH_OK, nullptr};
+    if (r->n_rot % 2 != 0 || r->n_rot > head_dim) return {LNH_ERR_INVALID, "the turned elements must be even in number and within the head"};
+    if (n_tokens == 0) return {LNH_OK, nullptr};
+    if (!r->device_angles) return {LNH_ERR_INVALID, "buffer pointer is null"};
+    if (attn_misaligned(r->device_angles, 8) || attn_misaligned(r->device_positions, 4))
+        return {LNH_ERR_INVALID, "angles must be 8-byte aligned, positions 4-byte aligned"};
+    if (r->angle_stride < r->n_rot / 2 || r->angle_stride > ((size_t)1 << 40)) return {LNH_ERR_INVALID, "a position's angles are fewer than its pairs, or 2^40 apart"};
+    if (r->n_positions == 0 || r->n_positions > ((size_t)1 << 31)) return {LNH_ERR_INVALID, "angles of no position, or of more than 2^31"};
+    return {LNH_OK, nullptr};
+}
+
+inline AttnCheck check_kv_append(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t layer, const lnh_rope *rope, size_t n_head, const float *q,
+                                 size_t q_stride, const float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v, size_t v_stride) {
+    AttnCheck r = check_kv_store(c, s, layer, k, k_stride, v, v_stride);
+    if (r.what) return r;
+    if (n_head > 65536) return {LNH_ERR_INVALID, "more than 65536 query heads"};
+    const bool rows = s->n_seqs != 0 && s->n_tokens != 0 && s->max_new != 0;
+    r = check_rope(rope, c->head_dim, rows ? s->n_tokens : 0);
+    if (r.what || !rows || n_head == 0) return r;
+    r = check_rows(q, q_stride, n_head * c->head_dim);
+    if (!r.what) r = check_rows(q_out, q_out_stride, n_head * c->head_dim);
+    if (!r.what && q == q_out && q_stride != q_out_stride) r = {LNH_ERR_INVALID, "rows turned in place have one stride"};
+    return r;
+}
+
+inline AttnCheck check_rope_table(uint32_t n_rot, double base, double scale, const float *divisors, size_t n_positions, const float *angles, size_t stride) {
+    if (n_rot == 0 || n_rot % 2 != 0) return {LNH_ERR_INVALID, "the turned elements must be even in number"};
+    if (!(base > 0 && base <= 1e300) || !(scale > 0 && scale <= 1e300)) return {LNH_ERR_INVALID, "base and scale must be positive and finite"};
+    if (n_positions > ((size_t)1 << 31)) return {LNH_ERR_INVALID, "angles of more than 2^31 positions"};
+    if (stride < n_rot / 2 || stride > ((size_t)1 << 40)) return {LNH_ERR_INVALID, "a position's angles are fewer than its pairs, or 2^40 apart"};
+    if (n_positions == 0) return {LNH_OK, nullptr};
+    if (!angles) return {LNH_ERR_INVALID, "buffer pointer is null"};
+    if (attn_misaligned(angles, 8) || attn_misaligned(divisors, 4)) return {LNH_ERR_INVALID, "angles must be 8-byte aligned, divisors 4-byte aligned"};
+    return {LNH_OK, nullptr};
 }
 
 inline AttnCheck check_kv_evict(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t first_layer, size_t n_layers, size_t keep, size_t first,
