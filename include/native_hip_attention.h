@@ -121,6 +121,26 @@ int lnh_attn_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs
                     const float *device_q, size_t q_stride, float *device_out, size_t out_stride, float scale,
                     size_t window, size_t sinks, int weights, float decay, void *stream);
 
+/* What the keys of a block of the cache lie between: the least and the largest value of each key element over the positions that the
+ * sequence has in the block, as device_bounds [n_blocks][n_layer][n_head_kv][2][head_dim] (16-byte aligned), f32 for an f32 cache, else f16:
+ * exactly numbers of the cache.  Formed anew, in `layer`, for every block that holds new tokens of the call, whose rows have to be
+ * stored before; a NaN among the values makes both bounds NaN.  Blocks that are not there are left out. */
+int lnh_kv_bounds_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, void *device_bounds, void *stream);
+
+/* lnh_attn_device over n_select blocks of the cache for each new token and key-value head, those that device_bounds (lnh_kv_bounds_device, of all
+ * blocks that the token sees whole) promise most of.  A block's score is the largest, over the query heads that share the key-value
+ * head, of the sum over the head's elements of q hi where q > 0 and q lo elsewhere - at least every product q k of the block -, formed
+ * in 64 bits and rounded to f32 (NaN counts as largest, a block that is not there as least).  A token at position p reads
+ * the positions up to p of the first `first` of its p / kv_block + 1 blocks, of the last `recent` (at least one, its own;
+ * first + recent <= n_select) and of those between them the ones of the largest score, ties to the lower; of all where they are
+ * no more than n_select.  device_chosen (may be NULL): which, [n_tokens][n_head_kv][n_select] in ascending order, 0xffffffff behind
+ * the last; rows that belong to no sequence are left as they are.  Otherwise as lnh_attn_device without window and weights, also in what it
+ * does with the executor's workspace: a word for every block of max_len, new token and key-value head, tokens in parts where that
+ * would pass 1 GiB. */
+int lnh_attn_select_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, size_t n_head, const void *device_bounds,
+                           size_t n_select, size_t first, size_t recent, const float *device_q, size_t q_stride, float *device_out,
+                           size_t out_stride, float scale, uint32_t *device_chosen, void *stream);
+
 /* Every sequence of more than `keep` positions is cut to `keep` of them, per layer (n_layers from first_layer on) and
  * key-value head: the first `first`, the last `recent` (first + recent <= keep) and of those between them the ones of
  * the largest device_w (NaN counts as largest, ties go to the lower position).  What stays moves together in its order

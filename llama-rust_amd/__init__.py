@@ -208,6 +208,8 @@ def load_library():
         "lnh_kv_append_device": (C.c_int, [vp, pc, ps, sz, pr, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp]),
         "lnh_kv_load_device": (C.c_int, [vp, pc, ps, sz, vp, sz, vp, sz, vp]),
         "lnh_attn_device": (C.c_int, [vp, pc, ps, sz, sz, vp, sz, vp, sz, C.c_float, sz, sz, C.c_int, C.c_float, vp]),
+        "lnh_kv_bounds_device": (C.c_int, [vp, pc, ps, sz, vp, vp]),
+        "lnh_attn_select_device": (C.c_int, [vp, pc, ps, sz, sz, vp, sz, sz, sz, vp, sz, vp, sz, C.c_float, vp, vp]),
         "lnh_kv_evict_device": (C.c_int, [vp, pc, ps, sz, sz, sz, sz, sz, vp, sz, vp, vp]),
     }
     for name, (res, args) in list(sig.items()) + list(paged.items()):
@@ -511,6 +513,19 @@ class HipGemv:
         row = n_head * cache.head_dim
         self._check(self._lib.lnh_attn_device(self._h, C.byref(cache), C.byref(seqs), layer, n_head, q_ptr, row if q_stride is None else q_stride,
                                               out_ptr, row if out_stride is None else out_stride, scale, window, sinks, int(weights), decay, stream))
+
+    def kv_bounds_device(self, cache, seqs, layer, bounds_ptr, stream=0):
+        """The least and largest key elements of every block that holds new tokens: bounds as [n_blocks][n_layer][n_head_kv][2][head_dim]."""
+        self._check(self._lib.lnh_kv_bounds_device(self._h, C.byref(cache), C.byref(seqs), layer, bounds_ptr, stream))
+
+    def attn_select_device(self, cache, seqs, layer, n_head, bounds_ptr, n_select, first, recent, q_ptr, out_ptr, scale, chosen_ptr=0, q_stride=None,
+                           out_stride=None, stream=0):
+        """attn_device over the n_select blocks that the bounds promise most of, for each new token and key-value head; chosen (0: not wanted):
+        which, [n_tokens][n_head_kv][n_select] u32."""
+        row = n_head * cache.head_dim
+        self._check(self._lib.lnh_attn_select_device(self._h, C.byref(cache), C.byref(seqs), layer, n_head, bounds_ptr, n_select, first, recent, q_ptr,
+                                                     row if q_stride is None else q_stride, out_ptr, row if out_stride is None else out_stride, scale,
+                                                     chosen_ptr, stream))
 
     def kv_evict_device(self, cache, seqs, first_layer, n_layers, keep, first, recent, dst_tables_ptr, dst_stride, new_lens_ptr, stream=0):
         """Every sequence to at most `keep` positions: the first, the recent, the heaviest between; dst_tables_ptr 0: in place."""

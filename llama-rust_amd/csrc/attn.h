@@ -47,10 +47,29 @@ struct AttnCall {
     size_t window, sinks;
     bool weights;
     float decay;
+    size_t head_tables;  // entries of a key-value head's own table, every row a sequence (launch_attn_select); else 0
 };
 // cus: compute units of the GPU.  ws holds at least *workspace bytes of the same call, 16-byte aligned.
 bool attn_fits(const AttnCall &c, uint32_t cus, size_t *workspace);
 hipError_t launch_attn(hipStream_t stream, const AttnCall &c, uint32_t cus, void *ws);
+
+struct KvBoundsCall {
+    const lnh_kv_cache *cache;
+    const lnh_kv_seqs *seqs;
+    size_t layer;
+    void *bounds;
+};
+bool kv_bounds_fits(const KvBoundsCall &c);
+hipError_t launch_kv_bounds(hipStream_t stream, const KvBoundsCall &c);
+
+struct AttnSelectCall {
+    AttnCall attn;  // no window, no weights
+    const void *bounds;
+    size_t n_select, first, recent;
+    uint32_t *chosen;  // may be null
+};
+bool attn_select_fits(const AttnSelectCall &c, uint32_t cus, size_t *workspace);
+hipError_t launch_attn_select(hipStream_t stream, const AttnSelectCall &c, uint32_t cus, void *ws);
 
 struct KvEvictCall {
     const lnh_kv_cache *cache;

@@ -32,6 +32,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 #include "kv_append.inc"
 #include "kv_store.inc"
 #include "kv_evict.inc"
+#include "kv_bounds.inc"
 
 KvPlace kv_place(const lnh_kv_cache &c, const uint32_t *tables, size_t stride) {
     KvPlace p;

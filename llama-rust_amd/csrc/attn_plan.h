@@ -255,6 +255,29 @@ inline AttnCheck check_rope_table(uint32_t n_rot, double base, double scale, con
     return {LNH_OK, nullptr};
 }
 
+inline AttnCheck check_kv_bounds(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t layer, const void *bounds) {
+    AttnCheck r = check_kv_cache(c, false);
+    if (!r.what) r = check_kv_seqs(c, s, true);
+    if (r.what) return r;
+    if (layer >= c->n_layer) return {LNH_ERR_INVALID, "the K/V cache has no such layer"};
+    if (s->n_seqs == 0 || s->n_tokens == 0 || s->max_new == 0) return {LNH_OK, nullptr};
+    if (!bounds) return {LNH_ERR_INVALID, "buffer pointer is null"};
+    if (attn_misaligned(bounds, 16)) return {LNH_ERR_INVALID, "device buffers must be 16-byte aligned"};
+    return {LNH_OK, nullptr};
+}
+
+inline AttnCheck check_attn_select(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t layer, size_t n_head, const void *bounds, size_t n_select, size_t first,
+                                   size_t recent, const float *q, size_t q_stride, const float *out, size_t out_stride, float scale, const uint32_t *chosen) {
+    AttnCheck r = check_attn(c, s, layer, n_head, q, q_stride, out, out_stride, scale, 0, 0, 0, 1.f);
+    if (!r.what) r = check_kv_bounds(c, s, layer, bounds);
+    if (r.what) return r;
+    if (recent == 0) return {LNH_ERR_INVALID, "a token's own block is always among those it reads: recent blocks are at least one"};
+    if (first > n_select || recent > n_select - first) return {LNH_ERR_INVALID, "first and recent blocks together exceed those to read"};
+    if (n_select > ATTN_MAX_POSITIONS / c->kv_block) return {LNH_ERR_INVALID, "the blocks to read exceed 31 bits of positions"};
+    if (attn_misaligned(chosen, 4)) return {LNH_ERR_INVALID, "chosen blocks must be 4-byte aligned"};
+    return {LNH_OK, nullptr};
+}
+
 inline AttnCheck check_kv_evict(const lnh_kv_cache *c, const lnh_kv_seqs *s, size_t first_layer, size_t n_layers, size_t keep, size_t first,
                                 size_t recent, const uint32_t *dst, size_t dst_stride, const uint32_t *new_lens) {
     AttnCheck r = check_kv_cache(c, true);

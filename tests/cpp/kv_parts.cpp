@@ -1,4 +1,4 @@
-// Checks before launches of the rotated append, the read back and the 4-bit cache (llama-rust_amd/csrc/attn_plan.h), with no device.
+// Checks before launches of the rotated append, the read back, the 4-bit cache and chosen blocks (llama-rust_amd/csrc/attn_plan.h), with no device.
 #include <cstdio>
 #include <initializer_list>
 #include <limits>
@@ -97,7 +97,48 @@ static void angles() {
     CHECK(code(64, 1e4, 1, SIZE_MAX, buf, 32) == LNH_ERR_INVALID);
 }
 
+static void chosen_blocks() {
+    struct Call {
+        lnh_kv_cache cache = good;
+        lnh_kv_seqs seqs = ::seqs;
+        size_t layer = 1, heads = 8, most = 4, first = 1, recent = 2, qs = 512, os = 512;
+        const void *bounds = buf + 512;
+        const float *q = buf, *out = buf + 1024;
+        float scale = 0.125f;
+        const uint32_t *chosen = idx;
+    };
+    const auto code = [](auto change) {
+        Call c;
+        change(c);
+        return nh::check_attn_select(&c.cache, &c.seqs, c.layer, c.heads, c.bounds, c.most, c.first, c.recent, c.q, c.qs, c.out, c.os, c.scale, c.chosen).code;
+    };
+    CHECK(code([](Call &) {}) == LNH_OK);
+    CHECK(code([](Call &c) { c.chosen = nullptr; }) == LNH_OK);
+    CHECK(code([](Call &c) { c.first = 2; }) == LNH_OK);
+    CHECK(code([](Call &c) { c.first = 3; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.first = SIZE_MAX; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.recent = SIZE_MAX; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.recent = 0; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.most = SIZE_MAX; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.most = nh::ATTN_MAX_POSITIONS / 16; }) == LNH_OK);
+    CHECK(code([](Call &c) { c.bounds = nullptr; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.bounds = buf + 1; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.chosen = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(idx) + 1); }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.heads = 6; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.layer = 2; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.scale = -1.f; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.out = c.q; }) == LNH_ERR_INVALID);
+    CHECK(code([](Call &c) { c.seqs.n_seqs = c.seqs.n_tokens = 0, c.bounds = c.q = c.out = nullptr; }) == LNH_OK);
+    CHECK(nh::check_kv_bounds(&good, &seqs, 0, buf).code == LNH_OK);
+    CHECK(nh::check_kv_bounds(&good, &seqs, 2, buf).code == LNH_ERR_INVALID);
+    CHECK(nh::check_kv_bounds(&good, &seqs, 0, nullptr).code == LNH_ERR_INVALID);
+    CHECK(nh::check_kv_bounds(&good, &seqs, 0, buf + 2).code == LNH_ERR_INVALID);
+    CHECK(nh::check_kv_bounds(nullptr, &seqs, 0, buf).code == LNH_ERR_INVALID);
+    CHECK(nh::check_kv_bounds(&good, nullptr, 0, buf).code == LNH_ERR_INVALID);
+}
+
 int main() {
+    chosen_blocks();
     four_bits();
     append();
     angles();

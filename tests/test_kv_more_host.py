@@ -1,4 +1,4 @@
-"""The rotated append, the read back and the 4-bit cache as far as no GPU is needed: their refusals, the structure's layout, the packing's own
+"""The rotated append, the read back, the 4-bit cache and chosen blocks as far as no GPU is needed: their refusals, the structure's layout, the packing's own
 properties."""
 import os
 import shutil
@@ -29,6 +29,8 @@ def test_no_executor_is_an_error(lib):
     assert lib.lnh_rope_table_device(None, 64, 1e4, 1.0, None, 1, None, 32, None) == 1
     assert lib.lnh_kv_append_device(None, None, None, 0, None, 0, None, 0, None, 0, None, 0, None, 0, None) == 1
     assert lib.lnh_kv_load_device(None, None, None, 0, None, 0, None, 0, None) == 1
+    assert lib.lnh_kv_bounds_device(None, None, None, 0, None, None) == 1
+    assert lib.lnh_attn_select_device(None, None, None, 0, 1, None, 1, 0, 1, None, 0, None, 0, 1.0, None, None) == 1
 
 
 def test_host_parts(tmp_path):
