@@ -149,6 +149,23 @@ def test_one_token_a_sequence(gpu, heads, hkv, d, block):
     assert np.all(got[1] == 0)
 
 
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("block", [32, 12, 6])
+@pytest.mark.parametrize("group", [3, 8, 9, 20])
+def test_heads_blocks_and_groups(gpu, d, block, group):
+    """Every way that rows are read, up to eight rows a head, more than eight, more than sixteen; shares of several tiles of every wavefront, blocks
+    that are not there and a window with first tokens among them."""
+    rng = np.random.default_rng(d + block)
+    c = Paged4(rng, 1, 1, d, block, [700, 45])
+    c.tables[0, 9] = NOWHERE
+    c.up()
+    q = rng.normal(0, 1, (2, group, d)).astype(np.float32)
+    scale = np.float32(d ** -0.5)
+    for window, sinks in ((0, 0), (90, 5)):
+        want, tol, _ = c.attend(0, q, float(scale), window=window, sinks=sinks)
+        check(attend(gpu, c, 0, q, scale, window=window, sinks=sinks), want, tol)
+
+
 @pytest.mark.parametrize("block", [1, 3, 8, 48, 256])
 def test_blocks_of_any_size(gpu, block):
     rng = np.random.default_rng(block)
