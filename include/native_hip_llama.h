@@ -77,14 +77,14 @@ int lnm_session_new(lnm_model *model, size_t kv_block, const uint32_t *block_ids
  * as a step; the environment variable LLAMA_HIP_DECODE_STEP_PREFILL makes every token a step. */
 int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,
                            size_t max_positions, lnm_session **out);
-/* The device session over the paged-cache operators of native_hip_attention.h: K and V are kept as kv_type (LNH_TYPE_F32, or
- * LNH_TYPE_F16: half the memory), a step's attention is shared by the whole GPU whatever the history (the session above gives
+/* The device session over the paged-cache operators of native_hip_attention.h: K and V are kept as kv_type (LNH_TYPE_F32,
+ * LNH_TYPE_F16: half the memory, or LNH_TYPE_Q4_0: a seventh), a step's attention is shared by the whole GPU whatever the history (the session above gives
  * each head one workgroup), a prompt's runs on the matrix cores, the block table may be of any length, and with window > 0 a token
  * sees the last `window` positions and the first `sinks` (every position stays in the cache).  Without a window and with f32,
  * results are the session above's but for the order of sums.  Four layers of 4096 columns, 32 heads of 128 over 8 (that
  * session, f32, f16): behind 128 positions a step takes 198, 219, 216 us (three launches a layer in place of one), behind 2048
  * 284, 238, 228, behind 16384 1222, 344, 290 and with a window of 1024 234; a prompt of 2048 17.9, 11.5, 11.0 ms, of 16384 1380,
- * 133, 91 ms.  Heads of a multiple of 8, at most 256.
+ * 133, 91 ms.  Heads of a multiple of 8 (LNH_TYPE_Q4_0: of 32), at most 256.
  * cache_positions (0: max_positions) bounds what the cache holds at a time.  weights != 0 (without a window): every layer and K/V head
  * sums the softmax weight each cached position has been given, for lnm_session_evict. */
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,

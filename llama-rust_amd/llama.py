@@ -170,7 +170,7 @@ class Llama:
         return out
 
     def session(self, kv_block=16, block_ids=None, device_positions=None, kv_type=None, window=0, sinks=0, cache_positions=0, weights=False):
-        """device_positions: keep the whole decode step on the GPU, with a cache of that many positions; kv_type (F32 or F16): over
+        """device_positions: keep the whole decode step on the GPU, with a cache of that many positions; kv_type (F32, F16 or Q4_0): over
         the paged-cache operators, a token seeing the last `window` positions (0: all) and the first `sinks`; cache_positions: a
         cache of fewer positions than the session has; weights: kept for evict()."""
         return Session(self, kv_block, block_ids, device_positions, kv_type, window, sinks, cache_positions, weights)
