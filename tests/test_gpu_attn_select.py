@@ -350,3 +350,22 @@ def test_refusals_touch_nothing(gpu, hip, pkg):
     none = pkg.KvSeqs(0, 0, 2, 0, 0, n_tokens=0)
     gpu.kv_bounds_device(c.cache, none, 0, 0)
     gpu.attn_select_device(c.cache, none, 0, 4, 0, 4, 1, 2, 0, 0, 0.125)
+
+
+@pytest.mark.parametrize("kind,heads,hkv,d,block", [("f16", 2, 2, 8, 16), ("q4_0", 33, 1, 64, 20)])
+def test_more_rows_than_a_launch_has_workgroups(gpu, hip, pkg, kind, heads, hkv, d, block):
+    """A prompt's rows in parts by the heads that they have (the check reads a few of them), its last token chosen for as if it were alone."""
+    rng = np.random.default_rng(12)
+    c = cache_of(kind, rng, 1, hkv, d, block, [3 * block])
+    n = (0x3fffff // hkv + 700) if heads == hkv else 300
+    c.up([0, n], max_new=n)  # all but the last 3 * block tokens are below position 0
+    q = np.zeros((n, heads, d), np.float32)
+    tail = rng.normal(0, 1, (3 * block, heads, d)).astype(np.float32)
+    q[n - 3 * block:] = tail
+    bounds = bounds_of(c, kind)
+    scale = d ** -0.5
+    want_chosen, want, tol = definition(c, kind, bounds, 0, tail, scale, [0, 3 * block], 2, 0, 1)
+    chosen, out = select(gpu, hip, c, bounds, 0, q, scale, 2, 0, 1)
+    assert np.array_equal(chosen[n - 3 * block:], want_chosen)
+    assert np.all(np.abs(out[n - 3 * block:] - want) <= tol + 1e-7 * np.abs(want))
+    assert np.all(out[:n - 3 * block] == 0)
