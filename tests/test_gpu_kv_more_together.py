@@ -111,6 +111,36 @@ def test_more_sequences_than_go_at_once(gpu, d, block, new, most):
     check(attend(gpu, c, 0, q, scale), want, tol + 1e-7 * np.abs(want))
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "q4_0"])
+@pytest.mark.parametrize("seqs,hkv,heads,d,new,most", [(277, 8, 8, 32, 1, 20), (131, 8, 16, 64, 1, 20), (67, 8, 64, 32, 3, 14), (277, 8, 8, 160, 1, 9), (300, 8, 8, 32, 1, 300)])
+def test_several_sequences_a_workgroup(gpu, kind, seqs, hkv, heads, d, new, most):
+    """Short sequences by the hundred, each some wavefronts of a workgroup, the last workgroup's not all there; some hold nothing, have places that are not there,
+    rows whose scores are computed again; the weights of a few query heads a key-value head from the scores that are kept."""
+    rng = np.random.default_rng(seqs + d)
+    lens = [int(x) for x in rng.integers(0, 15 if most == 300 else most, seqs)]
+    lens[5], lens[seqs - 2] = most, most - 1
+    weights = new == 1
+    c = (Paged4(rng, 1, hkv, d, 8, lens, weights=weights) if kind == "q4_0" else Paged(rng, kind == "f16", 1, hkv, d, 8, lens, weights=weights))
+    c.tables[6, 0] = c.n_blocks
+    starts = list(range(0, seqs * new + 1, new))
+    c.up(starts if new > 1 else None, max_new=new)
+    q = rng.normal(0, 1, (seqs * new, heads, d)).astype(np.float32)
+    q[::11] *= np.float32(1e6)
+    scale = np.float32(d ** -0.5)
+    want, tol, sums = c.attend(0, q, float(scale), starts)
+    got = attend(gpu, c, 0, q, scale)
+    check(got, want, tol + 1e-7 * np.abs(want))
+    assert np.array_equal(attend(gpu, c, 0, q, scale), got)
+    if weights:
+        assert np.array_equal(attend(gpu, c, 0, q, scale, weights=True, decay=0.5), got)
+        w, w_tol = c.weigh(0, sums, 0.5)
+        after = c.down()[2]
+        held = ~np.isnan(w)
+        assert same_bits(after[~held], c.w[~held])
+        off = np.abs(after[held] - w[held])
+        assert np.all(off <= w_tol[held]), np.max(off - w_tol[held])
+
+
 @pytest.mark.parametrize("new", [1, 24])
 def test_rows_of_nobody_and_blocks_of_several(gpu, hip, pkg, new):
     """A prefix that two sequences share, a block that stands twice in one table, rows before the first sequence and behind the last."""
