@@ -84,7 +84,7 @@ int lnm_session_new_device(lnm_model *model, size_t kv_block, const uint32_t *bl
  * results are the session above's but for the order of sums.  Four layers of 4096 columns, 32 heads of 128 over 8 (that
  * session, f32, f16): behind 128 positions a step takes 198, 219, 216 us (three launches a layer in place of one), behind 2048
  * 284, 238, 228, behind 16384 1222, 344, 290 and with a window of 1024 234; a prompt of 2048 17.9, 11.5, 11.0 ms, of 16384 1380,
- * 133, 91 ms.  Heads of a multiple of 8 (LNH_TYPE_Q4_0: of 32), at most 256.
+ * 133, 91 ms.  4 bits beside f16, another time: steps 222 and 228 us, 239 and 242, 269 and 295, prompts 12.6 and 12.2 ms, 97 and 96.  Heads of a multiple of 8 (LNH_TYPE_Q4_0: of 32), at most 256.
  * cache_positions (0: max_positions) bounds what the cache holds at a time.  weights != 0 (without a window): every layer and K/V head
  * sums the softmax weight each cached position has been given, for lnm_session_evict. */
 int lnm_session_new_device_paged(lnm_model *model, size_t kv_block, const uint32_t *block_ids, size_t n_block_ids,
