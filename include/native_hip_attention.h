@@ -136,7 +136,7 @@ int lnh_kv_bounds_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv
  * no more than n_select.  device_chosen (may be NULL): which, [n_tokens][n_head_kv][n_select] in ascending order, 0xffffffff behind
  * the last; rows that belong to no sequence are left as they are.  Otherwise as lnh_attn_device without window and weights, also in what it
  * does with the executor's workspace: a word for every block of max_len, new token and key-value head, tokens in parts where that
- * would pass 1 GiB. */
+ * would pass 1 GiB or a launch's workgroups.  A prompt of thousands of tokens may take longer so than by lnh_attn_device, whose tokens share what they read. */
 int lnh_attn_select_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, size_t n_head, const void *device_bounds,
                            size_t n_select, size_t first, size_t recent, const float *device_q, size_t q_stride, float *device_out,
                            size_t out_stride, float scale, uint32_t *device_chosen, void *stream);
