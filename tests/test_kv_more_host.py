@@ -46,7 +46,7 @@ def test_host_parts(tmp_path):
 
 
 def test_packing(pkg):
-    """What the checker packs: values are f16 exactly (unpack asserts it), within half a step unless they lie beyond seven of them, the same
+    """What the tests pack: values are f16 exactly (unpack asserts it), within half a step unless they lie beyond seven of them, the same
     when packed again; the buffer is the header's."""
     rng = np.random.default_rng(0)
     for size in (1e-6, 1.0, 1e4):
