@@ -3,7 +3,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
-#include "attn_plan.h"
+#include "attn_launch_plan.h"
 
 namespace nh {
 
@@ -36,21 +36,7 @@ hipError_t launch_kv_load(hipStream_t stream, const KvAppendCall &c, float *k, f
 hipError_t launch_rope_table(hipStream_t stream, uint32_t n_rot, double base, double scale, const float *divisors, size_t n_positions, float *angles,
                              size_t stride);
 
-struct AttnCall {
-    const lnh_kv_cache *cache;
-    const lnh_kv_seqs *seqs;
-    size_t layer, n_head;
-    const float *q;
-    float *out;
-    size_t q_stride, out_stride;
-    float scale;
-    size_t window, sinks;
-    bool weights;
-    float decay;
-    size_t head_tables;  // entries of a key-value head's own table, every row a sequence (launch_attn_select); else 0
-};
-// cus: compute units of the GPU.  ws holds at least *workspace bytes of the same call, 16-byte aligned.
-bool attn_fits(const AttnCall &c, uint32_t cus, size_t *workspace);
+// cus: compute units of the GPU.  ws holds at least what attn_fits() said of the same call, 16-byte aligned.
 hipError_t launch_attn(hipStream_t stream, const AttnCall &c, uint32_t cus, void *ws);
 
 struct KvBoundsCall {
@@ -62,13 +48,6 @@ struct KvBoundsCall {
 bool kv_bounds_fits(const KvBoundsCall &c);
 hipError_t launch_kv_bounds(hipStream_t stream, const KvBoundsCall &c);
 
-struct AttnSelectCall {
-    AttnCall attn;  // no window, no weights
-    const void *bounds;
-    size_t n_select, first, recent;
-    uint32_t *chosen;  // may be null
-};
-bool attn_select_fits(const AttnSelectCall &c, uint32_t cus, size_t *workspace);
 hipError_t launch_attn_select(hipStream_t stream, const AttnSelectCall &c, uint32_t cus, void *ws);
 
 struct KvEvictCall {
