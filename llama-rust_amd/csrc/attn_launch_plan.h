@@ -158,8 +158,11 @@ inline AttnPlan attn_plan(const AttnCall &c, uint32_t cus) {
         for (size_t n = 2; n <= waves; n *= 2)
             if (whole_us(n) < whole_us(side)) side = n;
         // shares: finding and joining them, and, once few compute units are left over, a round for every unit a compute unit with its tiles, half as many as
-        // of the longest, evenly (chosen blocks: as many)
-        const float shares_us = 11.5f + (6.f + (float)tiles / (chosen ? 1.f : 2.f) / waves * tile_us) * std::max((float)p.units / (float)cus - 0.2f, 0.f);
+        // of the longest, evenly (chosen blocks: as many).  Over f32 and f16 caches without that round up to half of the compute units, where a long
+        // sequence beside short ones would wait for its one workgroup (16 sequences of 30 positions and one of 700, f16: 10.5 us as shares, 13.5 whole;
+        // all of 700: 17.8 and 15.4)
+        const float load = (float)p.units / (float)cus, round_us = !packed && !chosen && load <= 0.5f ? 0.f : 6.f;
+        const float shares_us = 11.5f + (round_us + (float)tiles / (chosen ? 1.f : 2.f) / waves * tile_us) * std::max(load - 0.2f, 0.f);
         const bool soon = whole_us(side) <= shares_us;
         // shares count the tiles of all units together, in 32 bits
         const bool counted = c.seqs->max_len / tp + 2 <= 0x7fffffffu / p.units;
