@@ -124,7 +124,9 @@ int lnh_attn_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs
 /* What the keys of a block of the cache lie between: the least and the largest value of each key element over the positions that the
  * sequence has in the block, as device_bounds [n_blocks][n_layer][n_head_kv][2][head_dim] (16-byte aligned), f32 for an f32 cache, else f16:
  * exactly numbers of the cache.  Formed anew, in `layer`, for every block that holds new tokens of the call, whose rows have to be
- * stored before; a NaN among the values makes both bounds NaN.  Blocks that are not there are left out. */
+ * stored before; a NaN among the values makes both bounds NaN.  Blocks that are not there are left out.  Bounds hold as long as the rows of
+ * their block do: lnh_kv_evict_device moves rows to other blocks, and lnh_kv_bounds_device forms the bounds of the whole sequences again where
+ * every position counts as new - device_starts the running sum of the lengths, max_new = max_len, n_tokens at least the last start. */
 int lnh_kv_bounds_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t layer, void *device_bounds, void *stream);
 
 /* lnh_attn_device over n_select blocks of the cache for each new token and key-value head, those that device_bounds (lnh_kv_bounds_device, of all
@@ -149,8 +151,8 @@ int lnh_attn_select_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_
  * device_tables itself: in place.  Otherwise sequences that need no cut are copied as they are, and the destination's
  * blocks must be none that any of the call's sequences reads.  In place, sequences must not share blocks.  Rows behind
  * the new lengths are left as they are, and so is the new place of a position that stays though its block is not there: it is one of the
- * sequence's positions from then on.  device_starts is not looked at.  Uses the executor's workspace: a word a layer, key-value head and
- * position that may stay, sequences in parts as above. */
+ * sequence's positions from then on.  device_starts is not looked at.  Bounds (lnh_kv_bounds_device) of the blocks that it writes to hold no longer.  Uses
+ * the executor's workspace: a word a layer, key-value head and position that may stay, sequences in parts as above. */
 int lnh_kv_evict_device(lnh_exec *exec, const lnh_kv_cache *cache, const lnh_kv_seqs *seqs, size_t first_layer,
                         size_t n_layers, size_t keep, size_t first, size_t recent, const uint32_t *device_dst_tables,
                         size_t dst_stride, uint32_t *device_new_lens, void *stream);

@@ -528,7 +528,8 @@ class HipGemv:
                                                      chosen_ptr, stream))
 
     def kv_evict_device(self, cache, seqs, first_layer, n_layers, keep, first, recent, dst_tables_ptr, dst_stride, new_lens_ptr, stream=0):
-        """Every sequence to at most `keep` positions: the first, the recent, the heaviest between; dst_tables_ptr 0: in place."""
+        """Every sequence to at most `keep` positions: the first, the recent, the heaviest between; dst_tables_ptr 0: in place.  Bounds of the blocks
+        written to hold no longer: kv_bounds_device with every position as a new token forms them again."""
         self._check(self._lib.lnh_kv_evict_device(self._h, C.byref(cache), C.byref(seqs), first_layer, n_layers, keep, first, recent,
                                                   dst_tables_ptr, dst_stride, new_lens_ptr, stream))
 
