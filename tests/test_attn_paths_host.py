@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from attn_path_cases import F16, F32, LISTS_MANY, LISTS_SHARED, LISTS_WHOLE, PARTS, Q4_0, SHARED
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -23,9 +25,6 @@ def program(tmp_path_factory):
 def test_host_parts(program):
     r = subprocess.run([program], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.strip() == "OK", r.stdout + r.stderr
-
-
-F32, F16, Q4_0 = 0, 1, 2
 
 
 def paths(program, calls):
@@ -48,3 +47,14 @@ def paths(program, calls):
 def test_a_long_sequence_does_not_wait_for_one_workgroup(program, type, heads, heads_kv, dim, seqs, length, path):
     """Where a batch leaves half of the compute units idle, its longest sequence may be alone: it is shared out unless a workgroup has it done as soon."""
     assert paths(program, [dict(type=type, heads=heads, heads_kv=heads_kv, dim=dim, block=16, seqs=seqs, len=length)])[0].split()[0] == path
+
+
+@pytest.mark.parametrize("name,calls,kernel", [("shares", SHARED, "shares"), ("parts", PARTS, "shares"), ("lists, whole", LISTS_WHOLE, "whole"),
+                                               ("lists, shares", LISTS_SHARED, "shares"), ("lists, many rows", LISTS_MANY, "many")])
+def test_calls_take_the_kernels_they_are_tested_for(program, name, calls, kernel):
+    changes = [{}] if name != "shares" else [{}, dict(window=2500, sinks=40), dict(weights=True)]
+    for change in changes:
+        for call, path in zip(calls, paths(program, [dict(c, **change) for c in calls])):
+            assert path.split()[0] == kernel, (call, change, path)
+            if name == "parts":
+                assert int(path.split("parts=")[1]) > 1, (call, path)
